@@ -1,0 +1,78 @@
+/*
+ * nanollama_ops.h -- C ABI of libnanollama_stack.so, third part: operators on device memory.  A feed-forward of experts in three calls:
+ *
+ *   nl_op_route           scores of every expert -> the experts of every token and their weights
+ *   nl_op_experts         y = sum over a token's experts of weight * down(act(gate x) * up x), the tokens grouped by expert
+ *   nl_op_residual_norm   what closes a block: norm behind it, gate, residual scale, norm in front of the next
+ *
+ * The layer-stack models call the same kernels for layers that nl_stack_experts has given experts (below).
+ *
+ * Conventions.  Pointers are device memory of `device` that the caller owns, unless a comment says otherwise; nothing is kept behind a
+ * return, and no call allocates, synchronises or copies to the host: work is queued on `stream` (a hipStream_t of `device`, NULL: its
+ * default stream), and a call may be captured into a graph.  The caller's current device is as it was behind every call.  Arrays are
+ * row-major; ld* are elements from a row to the next.  n == 0 queues nothing.  Calls on different threads and streams do not disturb each
+ * other as long as their outputs and workspaces do not overlap.  0 or a negative nl_status; nl_last_error(NULL) has this thread's message.
+ * Element type `dtype`: NL_DTYPE_BF16 or NL_DTYPE_F32 (nanollama_stack.h); sums, scores, weights and norms are 32-bit either way.
+ */
+#ifndef NANOLLAMA_OPS_H
+#define NANOLLAMA_OPS_H
+
+#include "nanollama_stack.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+#define NL_MAX_EXPERTS 1024
+#define NL_MAX_PER_TOKEN 32
+
+enum { NL_SCORE_SOFTMAX = 0, NL_SCORE_SIGMOID = 1 };
+
+/* Which experts a token goes to.  An expert whose logit (or logit's place in `bias`) is -infinity or NaN is out.  Score s of the others:
+ *   NL_SCORE_SOFTMAX   exp(l) / sum of exp(l) over the row          chosen by l
+ *   NL_SCORE_SIGMOID   1 / (1 + exp(-l))                            chosen by l, or by s + bias
+ * The per_token largest, largest first, equal ones by lower number.  weight = scale * s, or scale * s / (sum of the chosen s) with renorm.
+ * Of logits of +infinity every one counts the same and the others nothing (softmax).  Places for which no expert is left get id -1 and
+ * weight 0. */
+typedef struct {
+    int32_t experts, per_token;   /* per_token <= min(experts, NL_MAX_PER_TOKEN) */
+    int32_t score;                /* NL_SCORE_* */
+    int32_t renorm;
+    float scale;
+} nl_route_desc;
+/* logits [n][ld], bias [experts] or NULL (sigmoid scores only), ids and weights [n][per_token]. */
+NL_API int nl_op_route(int device, void *stream, const nl_route_desc *d, int n, const float *logits, int64_t ld, const float *bias,
+                       int32_t *ids, float *weights);
+
+typedef struct {
+    int32_t experts, per_token;
+    int32_t dim, ff;              /* width of tokens, width of an expert */
+    int32_t act;                  /* NL_ACT_* */
+    int32_t dtype;                /* of x, the matrices and y */
+} nl_experts_desc;
+/* x [n][ldx], ids and weights [n][per_token], gate and up [experts][ff][dim], down [experts][dim][ff], y [n][ldy].  An id outside
+ * [0, experts) adds nothing, whatever its weight (a row without any: y = 0); an id twice in a row counts twice.  Rows of y behind n are
+ * not touched.  bfloat16: the activation and y are rounded, nothing else is.  Rows that start on 16-byte boundaries (pointers, and dim, ff, ldx times the element's size) take 16-byte loads; others are correct and slow.
+ * workspace: at least nl_op_experts_workspace bytes, on a 16-byte boundary, this call's alone until its work is done (two graphs that may
+ * run at the same time need one each).  x and y must not overlap. */
+NL_API int nl_op_experts(int device, void *stream, const nl_experts_desc *d, int n, const void *x, int64_t ldx, const int32_t *ids,
+                         const float *weights, const void *gate, const void *up, const void *down, void *y, int64_t ldy, void *workspace,
+                         uint64_t workspace_bytes);
+/* bytes for calls of up to n tokens (host arithmetic); 0: the description is not one that nl_op_experts takes */
+NL_API uint64_t nl_op_experts_workspace(const nl_experts_desc *d, int n);
+
+/* x_out = x + scale * gate * v,  v = norm(d) * post, or d without post;    h = norm(x_out) * pre  (h NULL: not asked for)
+ * norm(v) = v / sqrt(mean(v^2) + eps).  x, x_out: 32-bit; d, h: dtype.  gate: 32-bit, one row for all (ldgate 0) or a row a token; NULL: 1.
+ * post, pre: 32-bit gains [dim].  x_out may be x; no other overlap. */
+typedef struct {
+    int32_t dim, dtype;
+    float eps, scale;
+} nl_residual_norm_desc;
+NL_API int nl_op_residual_norm(int device, void *stream, const nl_residual_norm_desc *d, int n, const float *x, int64_t ldx, const void *b,
+                               int64_t ldb, const float *post, const float *gate, int64_t ldgate, const float *pre, float *x_out,
+                               int64_t ldxo, void *h, int64_t ldh);
+
+#ifdef __cplusplus
+}
+#endif
+#endif /* NANOLLAMA_OPS_H */

@@ -61,6 +61,21 @@ class NlLayerDesc(C.Structure):
     _fields_ = [("attn", NlAttnDesc), ("lin", NlLinattnDesc), ("latent", NlLatentDesc)] + [(n, C.c_int32) for n in ("ff", "ff_act", "ff_bias")]
 
 
+class NlRouteDesc(C.Structure):
+    """nl_route_desc: which experts a token goes to."""
+    _fields_ = [(n, C.c_int32) for n in ("experts", "per_token", "score", "renorm")] + [("scale", C.c_float)]
+
+
+class NlExpertsDesc(C.Structure):
+    """nl_experts_desc: sizes of a feed-forward of experts."""
+    _fields_ = [(n, C.c_int32) for n in ("experts", "per_token", "dim", "ff", "act", "dtype")]
+
+
+class NlResidualNormDesc(C.Structure):
+    """nl_residual_norm_desc: what closes a block."""
+    _fields_ = [("dim", C.c_int32), ("dtype", C.c_int32), ("eps", C.c_float), ("scale", C.c_float)]
+
+
 class NlStackConfig(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("vocab", "dim", "n_layers", "loop_start", "loop_stop", "loop_times", "seq_len", "max_streams",
                                          "max_step_tokens", "device", "dtype", "flags", "plain_norm", "post_norm", "untied")] + \
@@ -73,8 +88,8 @@ class NlError(RuntimeError):
         self.code = code
 
 
-_STACK_ONLY = ("nl_latent.h", "nl_linattn.h", "nl_mfma.h", "nl_winattn.h")
-_STACK_HEADERS = ("nl_kernels.h", "nl_latent.h", "nl_linattn.h", "nl_mfma.h", "nl_sample.h", "nl_winattn.h")
+_STACK_ONLY = ("nl_experts.h", "nl_frag.h", "nl_latent.h", "nl_linattn.h", "nl_mfma.h", "nl_ops.h", "nl_winattn.h")
+_STACK_HEADERS = ("nl_experts.h", "nl_frag.h", "nl_kernels.h", "nl_latent.h", "nl_linattn.h", "nl_mfma.h", "nl_ops.h", "nl_sample.h", "nl_winattn.h")
 
 
 def source_files(family: str = "hip"):
@@ -82,7 +97,7 @@ def source_files(family: str = "hip"):
     root, src_dir = os.path.dirname(_HERE), os.path.join(_HERE, "csrc")
     inc = lambda *names: [os.path.join(root, "include", n) for n in names]
     if family == "stack":
-        return [os.path.join(src_dir, f) for f in ("nl_stack.hip",) + _STACK_HEADERS] + inc("nanollama_hip.h", "nanollama_stack.h")
+        return [os.path.join(src_dir, f) for f in ("nl_stack.hip", "nl_ops.hip") + _STACK_HEADERS] + inc("nanollama_hip.h", "nanollama_stack.h", "nanollama_ops.h")
     hdrs = sorted(f for f in os.listdir(src_dir) if f.endswith(".h") and f not in _STACK_ONLY)
     return [os.path.join(src_dir, f) for f in ["nl_engine.hip"] + hdrs] + inc("nanollama_hip.h")
 
@@ -118,7 +133,7 @@ def build(force: bool = False, family: str = "hip") -> str:
             stale = f"src={source_sha(files)} git=".encode() not in fh.read()
     if force or stale:
         target = "../libnanollama_hip.so" if family == "hip" else "../libnanollama_stack.so"
-        subprocess.check_call(["make", "-C", src_dir, "-B", target], stdout=sys.stderr)
+        subprocess.check_call(["make", "-C", src_dir, "-j2", "-B", target], stdout=sys.stderr)
     return path
 
 
@@ -137,7 +152,8 @@ EXPORTS = ["nl_build_info", "nl_set_gamma", "nl_abi_version", "nl_device_count",
 STACK_EXPORTS = ["nl_build_info", "nl_abi_version", "nl_device_count", "nl_create_stack", "nl_upload_tensor", "nl_finalize", "nl_destroy",
                  "nl_last_error", "nl_reset", "nl_forward", "nl_forward_argmax", "nl_decode_greedy", "nl_prefill", "nl_forward_batch",
                  "nl_get_config", "nl_synchronize", "nl_timer_start", "nl_timer_stop", "nl_memory_usage", "nl_debug_read",
-                 "nl_sample_decode", "nl_host_logits", "nl_step", "nl_trace_layers"]
+                 "nl_sample_decode", "nl_host_logits", "nl_step", "nl_trace_layers", "nl_op_route", "nl_op_experts",
+                 "nl_op_experts_workspace", "nl_op_residual_norm"]
 
 _vp, _i32, _fp, _ip = C.c_void_p, C.c_int, C.POINTER(C.c_float), C.POINTER(C.c_int)
 
@@ -221,6 +237,12 @@ def stack_lib():
         L.nl_create_stack.argtypes = [C.POINTER(NlStackConfig), C.POINTER(NlLayerDesc), C.POINTER(_vp)]
         L.nl_step.argtypes = [_vp, _i32, _ip, _ip, _ip, _ip, _i32, _ip, _fp, _ip]
         L.nl_trace_layers.argtypes = [_vp, _i32]
+        L.nl_op_route.argtypes = [_i32, _vp, C.POINTER(NlRouteDesc), _i32, _vp, C.c_int64, _vp, _vp, _vp]
+        L.nl_op_experts.argtypes = [_i32, _vp, C.POINTER(NlExpertsDesc), _i32, _vp, C.c_int64] + [_vp] * 6 + [C.c_int64, _vp, C.c_uint64]
+        L.nl_op_experts_workspace.argtypes = [C.POINTER(NlExpertsDesc), _i32]
+        L.nl_op_experts_workspace.restype = C.c_uint64
+        L.nl_op_residual_norm.argtypes = [_i32, _vp, C.POINTER(NlResidualNormDesc), _i32, _vp, C.c_int64, _vp, C.c_int64, _vp, _vp, C.c_int64, _vp, _vp,
+                                          C.c_int64, _vp, C.c_int64]
         _stack = L
     return _stack
 

@@ -1,0 +1,191 @@
+// nl_ops.hip -- host side of the operators on device memory (include/nanollama_ops.h): checks, launches, the rules by which a kernel is chosen.
+#include "nl_experts.h"
+
+#include <climits>
+#include <cstdarg>
+#include <cstdio>
+#include <algorithm>
+#include <tuple>
+
+using namespace nl;
+
+namespace {
+
+template <typename... F, typename... A>
+hipError_t start(void (*kernel)(F...), dim3 grid, dim3 block, size_t lds, hipStream_t st, A... args) {
+    static_assert(sizeof...(F) == sizeof...(A), "kernel arguments");
+    std::tuple<F...> held(args...);
+    void *at[sizeof...(F)];
+    std::apply([&](auto &...a) { int i = 0; ((at[i++] = (void *)&a), ...); }, held);
+    return hipLaunchKernel(reinterpret_cast<const void *>(kernel), grid, block, at, lds, st);
+}
+
+inline bool on16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+}  // namespace
+
+namespace nl {
+
+hipError_t launch_route(const RouteParams &P, hipStream_t st) {
+    const dim3 grid((P.n + 3) / 4), block(256);
+    const int ne = (P.experts + 63) / 64;
+    if (ne <= 1) return start(route_kernel<1>, grid, block, 0, st, P);
+    if (ne <= 2) return start(route_kernel<2>, grid, block, 0, st, P);
+    if (ne <= 4) return start(route_kernel<4>, grid, block, 0, st, P);
+    if (ne <= 8) return start(route_kernel<8>, grid, block, 0, st, P);
+    return start(route_kernel<16>, grid, block, 0, st, P);
+}
+
+ExpertsLayout experts_layout(int n, int k, int experts, int dim, int ff, int dtype) {
+    const size_t slots = (size_t)n * k, es = dtype == NL_DTYPE_F32 ? 4 : 2;
+    auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
+    ExpertsLayout L;
+    L.offs = 0;
+    L.order = up((size_t)(experts + 1) * 4);
+    L.h = L.order + up(slots * 4);
+    L.part = L.h + up(slots * ff * es);
+    L.bytes = L.part + up(slots * dim * 4);
+    return L;
+}
+
+template <typename T> static hipError_t experts(const ExpertsParams &P, hipStream_t st) {
+    const int slots = P.n * P.k;
+    hipError_t rc = start(plan_kernel, dim3(P.experts), dim3(1024), 0, st, P.ids, slots, P.experts, P.offs, P.order);
+    if (rc != hipSuccess) return rc;
+    constexpr int W = 16 / (int)sizeof(T);               // elements of a 16-byte piece
+    const bool vec = on16(P.x) && on16(P.gate) && on16(P.up) && on16(P.down) && P.ldx % W == 0 && P.dim % W == 0 && P.ff % W == 0;
+    const int hit = std::min(P.experts, slots), tiles = hit + (slots - hit) / 16;
+    constexpr int R = 2;
+    const dim3 g1((P.ff + 16 * R - 1) / (16 * R), tiles), g2((P.dim + 16 * R - 1) / (16 * R), tiles);
+    if (vec) {
+        if ((rc = start(experts_few_kernel<T, true, true, R>, g1, dim3(256), 0, st, P)) != hipSuccess) return rc;
+        return start(experts_few_kernel<T, false, true, R>, g2, dim3(256), 0, st, P);
+    }
+    if ((rc = start(experts_few_kernel<T, true, false, R>, g1, dim3(256), 0, st, P)) != hipSuccess) return rc;
+    return start(experts_few_kernel<T, false, false, R>, g2, dim3(256), 0, st, P);
+}
+hipError_t launch_experts(const ExpertsParams &P, int dtype, hipStream_t st) { return dtype == NL_DTYPE_F32 ? experts<float>(P, st) : experts<bf16>(P, st); }
+
+hipError_t launch_close(const CloseParams &P, int dtype, hipStream_t st) {
+    return dtype == NL_DTYPE_F32 ? start(close_kernel<float>, dim3(P.n), dim3(256), 0, st, P) : start(close_kernel<bf16>, dim3(P.n), dim3(256), 0, st, P);
+}
+
+}  // namespace nl
+
+// ================================================================== C ABI ===
+
+namespace {
+
+int fail(int code, const char *fmt, ...) {
+    char buf[256];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof buf, fmt, ap);
+    va_end(ap);
+    set_error(buf);
+    return code;
+}
+
+// the caller's current device, given back at the end
+struct OnDevice {
+    int before = -1;
+    hipError_t rc;
+    explicit OnDevice(int device) {
+        if ((rc = hipGetDevice(&before)) == hipSuccess && before != device) rc = hipSetDevice(device);
+        else if (rc == hipSuccess) before = -1;          // nothing to give back
+    }
+    ~OnDevice() { if (before >= 0) (void)hipSetDevice(before); }
+    OnDevice(const OnDevice &) = delete;
+};
+
+// what every operator checks behind its own arguments, then the launches
+template <typename F> int on_device(const char *name, int device, void *stream, F launches) {
+    int ndev = 0;
+    if (hipGetDeviceCount(&ndev) != hipSuccess || ndev == 0) return fail(NL_ERR_HIP, "%s: no HIP device", name);
+    if (device < 0 || device >= ndev) return fail(NL_ERR_INVALID, "%s: device %d of %d", name, device, ndev);
+    OnDevice on(device);
+    if (on.rc != hipSuccess) return fail(NL_ERR_HIP, "%s: %s", name, hipGetErrorString(on.rc));
+    const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    hipDevice_t at = device;
+    if (st && hipStreamGetDevice(st, &at) == hipSuccess && at != device) return fail(NL_ERR_INVALID, "%s: the stream is of device %d, not %d", name, at, device);
+    const hipError_t rc = launches(st);
+    return rc == hipSuccess ? (int)NL_OK : fail(NL_ERR_HIP, "%s: %s", name, hipGetErrorString(rc));
+}
+
+const char *experts_error(const nl_experts_desc *d, int n) {
+    if (!d) return "no description";
+    if (d->experts < 1 || d->experts > NL_MAX_EXPERTS) return "experts: 1 to 1024";
+    if (d->per_token < 1 || d->per_token > NL_MAX_PER_TOKEN) return "per_token: 1 to 32";
+    if (d->dim < 1 || d->ff < 1 || d->dim > 1 << 20 || d->ff > 1 << 20) return "dim and ff: 1 to 1048576";
+    if (d->act != NL_ACT_SILU && d->act != NL_ACT_GELU_TANH) return "act";
+    if (d->dtype != NL_DTYPE_BF16 && d->dtype != NL_DTYPE_F32) return "dtype";
+    if (n < 0 || (long long)n * d->per_token > INT_MAX / 2) return "n: 0 to 2^30 / per_token";
+    return nullptr;
+}
+
+}  // namespace
+
+extern "C" {
+
+int nl_op_route(int device, void *stream, const nl_route_desc *d, int n, const float *logits, int64_t ld, const float *bias, int32_t *ids, float *weights) {
+    if (!d || n < 0) return fail(NL_ERR_INVALID, "route: %s", d ? "n is negative" : "no description");
+    if (d->experts < 1 || d->experts > NL_MAX_EXPERTS) return fail(NL_ERR_UNSUPPORTED, "route: %d experts, 1 to %d are taken", d->experts, NL_MAX_EXPERTS);
+    if (d->per_token < 1 || d->per_token > NL_MAX_PER_TOKEN || d->per_token > d->experts)
+        return fail(NL_ERR_INVALID, "route: %d per token, 1 to %d are taken, no more than experts", d->per_token, NL_MAX_PER_TOKEN);
+    if (d->score != NL_SCORE_SOFTMAX && d->score != NL_SCORE_SIGMOID) return fail(NL_ERR_INVALID, "route: score %d", d->score);
+    if (bias && d->score != NL_SCORE_SIGMOID) return fail(NL_ERR_UNSUPPORTED, "route: a bias goes with sigmoid scores");
+    if (!(d->scale - d->scale == 0.f)) return fail(NL_ERR_INVALID, "route: scale is not finite");
+    if (n == 0) return NL_OK;
+    if (!logits || !ids || !weights) return fail(NL_ERR_INVALID, "route: null argument");
+    if (ld < d->experts) return fail(NL_ERR_INVALID, "route: ld %lld is less than %d experts", (long long)ld, d->experts);
+    RouteParams P{};
+    P.logits = logits; P.bias = bias; P.ld = ld; P.n = n; P.experts = d->experts; P.k = d->per_token; P.sigmoid = d->score == NL_SCORE_SIGMOID;
+    P.renorm = d->renorm != 0; P.scale = d->scale; P.ids = ids; P.weights = weights;
+    return on_device("route", device, stream, [&](hipStream_t st) { return launch_route(P, st); });
+}
+
+uint64_t nl_op_experts_workspace(const nl_experts_desc *d, int n) {
+    if (const char *m = experts_error(d, n)) { fail(NL_ERR_INVALID, "experts: %s", m); return 0; }
+    return experts_layout(n, d->per_token, d->experts, d->dim, d->ff, d->dtype).bytes;
+}
+
+int nl_op_experts(int device, void *stream, const nl_experts_desc *d, int n, const void *x, int64_t ldx, const int32_t *ids, const float *weights,
+                  const void *gate, const void *up, const void *down, void *y, int64_t ldy, void *workspace, uint64_t workspace_bytes) {
+    if (const char *m = experts_error(d, n)) return fail(NL_ERR_INVALID, "experts: %s", m);
+    if (n == 0) return NL_OK;
+    if (!x || !ids || !weights || !gate || !up || !down || !y || !workspace) return fail(NL_ERR_INVALID, "experts: null argument");
+    if (ldx < d->dim || ldy < d->dim) return fail(NL_ERR_INVALID, "experts: ldx %lld and ldy %lld, rows have %d elements", (long long)ldx, (long long)ldy, d->dim);
+    const ExpertsLayout L = experts_layout(n, d->per_token, d->experts, d->dim, d->ff, d->dtype);
+    if (workspace_bytes < L.bytes) return fail(NL_ERR_INVALID, "experts: workspace of %llu bytes, %llu are needed", (unsigned long long)workspace_bytes, (unsigned long long)L.bytes);
+    if (!on16(workspace)) return fail(NL_ERR_INVALID, "experts: workspace is not on a 16-byte boundary");
+    char *ws = reinterpret_cast<char *>(workspace);
+    ExpertsParams P{};
+    P.x = x; P.gate = gate; P.up = up; P.down = down; P.ldx = ldx; P.ids = ids; P.weights = weights; P.n = n; P.k = d->per_token; P.experts = d->experts;
+    P.dim = d->dim; P.ff = d->ff; P.act = d->act;
+    P.offs = reinterpret_cast<int *>(ws + L.offs); P.order = reinterpret_cast<int *>(ws + L.order); P.h = ws + L.h; P.part = reinterpret_cast<float *>(ws + L.part);
+    CloseParams C{};
+    C.part = P.part; C.ids = ids; C.k = P.k; C.experts = P.experts; C.y = y; C.ldy = ldy; C.n = n; C.dim = d->dim;
+    return on_device("experts", device, stream, [&](hipStream_t st) {
+        const hipError_t rc = launch_experts(P, d->dtype, st);
+        return rc != hipSuccess ? rc : launch_close(C, d->dtype, st);
+    });
+}
+
+int nl_op_residual_norm(int device, void *stream, const nl_residual_norm_desc *d, int n, const float *x, int64_t ldx, const void *b, int64_t ldb, const float *post,
+                        const float *gate, int64_t ldgate, const float *pre, float *x_out, int64_t ldxo, void *h, int64_t ldh) {
+    if (!d || n < 0) return fail(NL_ERR_INVALID, "residual_norm: %s", d ? "n is negative" : "no description");
+    if (d->dim < 1 || d->dim > 1 << 20) return fail(NL_ERR_INVALID, "residual_norm: dim %d, 1 to %d are taken", d->dim, 1 << 20);
+    if (d->dtype != NL_DTYPE_BF16 && d->dtype != NL_DTYPE_F32) return fail(NL_ERR_INVALID, "residual_norm: dtype %d", d->dtype);
+    if (!(d->eps >= 0.f) || !(d->eps - d->eps == 0.f) || !(d->scale - d->scale == 0.f)) return fail(NL_ERR_INVALID, "residual_norm: eps or scale");
+    if (n == 0) return NL_OK;
+    if (!x || !b || !x_out || (h && !pre)) return fail(NL_ERR_INVALID, "residual_norm: null argument");
+    if (ldx < d->dim || ldb < d->dim || ldxo < d->dim || (gate && ldgate != 0 && ldgate < d->dim) || (h && ldh < d->dim))
+        return fail(NL_ERR_INVALID, "residual_norm: a row distance is less than %d", d->dim);
+    if (x_out == x && ldxo != ldx) return fail(NL_ERR_INVALID, "residual_norm: x_out is x with other rows");
+    CloseParams P{};
+    P.x = x; P.ldx = ldx; P.d = b; P.ldd = ldb; P.post = post; P.gate = gate; P.ldgate = ldgate; P.pre = pre; P.x_out = x_out; P.ldxo = ldxo; P.h = h; P.ldh = ldh;
+    P.n = n; P.dim = d->dim; P.eps = d->eps; P.scale = d->scale;
+    return on_device("residual_norm", device, stream, [&](hipStream_t st) { return launch_close(P, d->dtype, st); });
+}
+
+}  // extern "C"

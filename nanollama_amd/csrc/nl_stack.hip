@@ -16,6 +16,7 @@
 #include "../../include/nanollama_stack.h"
 #include "nl_sample.h"
 #include "nl_latent.h"
+#include "nl_ops.h"
 
 #include <algorithm>
 #include <cmath>
@@ -780,6 +781,12 @@ int run_decode(nl_engine *e, const int *streams, const int *tokens, const int *p
 }
 
 }  // namespace
+
+namespace nl {
+void set_error(const char *message) {
+    try { g_create_error = message; } catch (...) {}
+}
+}  // namespace nl
 
 // ================================================================== C ABI ===
 
