@@ -187,63 +187,55 @@ __global__ void __launch_bounds__(1024) plan_kernel(const int *ids, int nslots, 
     }
 }
 
-// tile number `tile` of the experts' places cut into tiles of BT: expert, first place, places; false: there are not that many.
-// Every wavefront finds it by itself: a lane counts the tiles of a run of experts, a scan finds the lane.
+// The experts' places cut into tiles of BT, an expert's tiles one behind the other: which expert has tile `tile`, how many tiles are in front of
+// its first one, its places [a, b).  Every wavefront finds it by itself: a lane counts the tiles of a run of experts, a scan finds the lane.
+struct Group { int e, before, a, b; };
 template <int BT>
-__device__ __forceinline__ bool find_tile(const int *offs, int experts, int tile, int &e, int &first, int &count) {
-    const int lane = threadIdx.x & 63, per = (experts + 63) >> 6, e0 = lane * per;
-    int mine = 0, lo = offs[min(e0, experts)];
-    for (int i = 0, a = lo; i < per; i++) {
-        const int b = offs[min(e0 + i + 1, experts)];
-        mine += (b - a + BT - 1) / BT;
-        a = b;
-    }
-    int upto = mine;
+struct Groups {
+    int per, mine, upto;
+    const int *offs;
+    __device__ __forceinline__ Groups(const int *o, int experts) : offs(o) {
+        const int lane = threadIdx.x & 63, e0 = lane * (per = (experts + 63) >> 6);
+        mine = 0;
+        for (int i = 0, a = offs[min(e0, experts)]; i < per; i++) {
+            const int b = offs[min(e0 + i + 1, experts)];
+            mine += (b - a + BT - 1) / BT;
+            a = b;
+        }
+        upto = mine;
 #pragma unroll
-    for (int s = 1; s < 64; s <<= 1) {
-        const int o = __shfl_up(upto, s);
-        if (lane >= s) upto += o;
+        for (int s = 1; s < 64; s <<= 1) {
+            const int o2 = __shfl_up(upto, s);
+            if (lane >= s) upto += o2;
+        }
     }
-    const unsigned long long who = __ballot(upto > tile);
-    if (!who) return false;
-    const int at = __ffsll((long long)who) - 1;
-    int skip = tile - __builtin_amdgcn_readlane(upto - mine, at);
-    e = at * per;
-    int a = __builtin_amdgcn_readfirstlane(offs[e]);
-    for (;; e++) {
-        const int b = __builtin_amdgcn_readfirstlane(offs[e + 1]), n = (b - a + BT - 1) / BT;
-        if (skip < n) { first = a + skip * BT; count = min(BT, b - first); return true; }
-        skip -= n;
-        a = b;
+    __device__ __forceinline__ int total() const { return __builtin_amdgcn_readlane(upto, 63); }
+    __device__ __forceinline__ Group find(int tile) const {          // tile < total()
+        const int at = __ffsll((long long)__ballot(upto > tile)) - 1;
+        Group G;
+        G.before = __builtin_amdgcn_readlane(upto - mine, at);
+        G.e = at * per;
+        G.a = __builtin_amdgcn_readfirstlane(offs[G.e]);
+        for (;;) {
+            G.b = __builtin_amdgcn_readfirstlane(offs[G.e + 1]);
+            const int n = (G.b - G.a + BT - 1) / BT;
+            if (tile - G.before < n) return G;
+            G.before += n;
+            G.a = G.b;
+            G.e++;
+        }
     }
-}
+};
 
 // ------------------------------------------------------------- products ---
 
-// a lane's run of 8 elements from k0 on of a row of K, zero behind its end.  VEC: 16-byte pieces, which lie within the row or behind it
-template <bool VEC> __device__ __forceinline__ Frag<bf16> load_run(const bf16 *row, int k0, int K) {
-    Frag<bf16> f;
+// a lane's run of 8 elements from k0 on of a row of K, zero behind its end
+template <typename T> __device__ __forceinline__ Frag<T> load_run(const T *row, int k0, int K) {
+    Frag<T> f;
     frag_zero(f);
-    if constexpr (VEC) {
-        if (k0 < K) f.v = *reinterpret_cast<const bf16x8 *>(row + k0);
-    } else {
 #pragma unroll
-        for (int j = 0; j < 8; j++)
-            if (k0 + j < K) f.v[j] = row[k0 + j];
-    }
-    return f;
-}
-template <bool VEC> __device__ __forceinline__ Frag<float> load_run(const float *row, int k0, int K) {
-    Frag<float> f;
-    frag_zero(f);
-    if constexpr (VEC) {
-        if (k0 < K) f.a = *reinterpret_cast<const f32x4 *>(row + k0);
-        if (k0 + 4 < K) f.b = *reinterpret_cast<const f32x4 *>(row + k0 + 4);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; j++)
-            if (k0 + j < K) frag_set(f, j, row[k0 + j]);
-    }
+    for (int j = 0; j < 8; j++)
+        if (k0 + j < K) frag_set(f, j, (float)row[k0 + j]);
     return f;
 }
 template <typename T> __device__ __forceinline__ void put_rows(T *p, int row, int rows, f32x4 v) {     // four consecutive ones, those that exist
@@ -260,43 +252,241 @@ template <bool SILU> __device__ __forceinline__ f32x4 activate(f32x4 gate, f32x4
     return v;
 }
 
-// 16 places x 16 R rows of one expert by a workgroup, K dealt to its four wavefronts, fragments straight to registers.  FIRST: gate and up rows of
-// the tokens -> h; else rows of down of h -> part
+// Rows that do not start on 16-byte boundaries: 16 places x 32 rows of one expert by a workgroup, K dealt to its four wavefronts, elements one by one
+// straight to registers (about ten times as long as with 16-byte pieces).  FIRST: gate and up rows of the tokens -> h; else rows of down of h -> part
 // (32-bit: a third rounding to bfloat16, beside the activation's and the sum's, would make the error 1.2 times as large: 2.9e-3 instead of 2.4e-3).
-template <typename T, bool FIRST, bool VEC, int R>
-__global__ void __launch_bounds__(256) experts_few_kernel(ExpertsParams P) {
-    constexpr int M = FIRST ? 2 : 1, N = R * M;
+template <typename T, bool FIRST>
+__global__ void __launch_bounds__(256) experts_any_kernel(ExpertsParams P) {
+    constexpr int R = 2, M = FIRST ? 2 : 1, N = R * M;
     __shared__ __align__(16) f32x4 red[4][N][64];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
     const int rows = FIRST ? P.ff : P.dim, K = FIRST ? P.dim : P.ff, row0 = blockIdx.x * 16 * R;
-    int e, first, count;
-    if (!find_tile<16>(P.offs, P.experts, blockIdx.y, e, first, count)) return;
-    const int place = first + min(c, count - 1), slot = P.order[place];
-    const T *x = FIRST ? reinterpret_cast<const T *>(P.x) + (long long)(slot / P.k) * P.ldx : reinterpret_cast<const T *>(P.h) + (long long)place * P.ff;
-    const T *a[N];
+    const Groups<16> groups(P.offs, P.experts);
+    for (int tile = blockIdx.y; tile < groups.total(); tile += gridDim.y) {
+        const Group G = groups.find(tile);
+        const int e = G.e, first = G.a + (tile - G.before) * 16, count = min(16, G.b - first);
+        const int place = first + min(c, count - 1), slot = P.order[place];
+        const T *x = FIRST ? reinterpret_cast<const T *>(P.x) + (long long)(slot / P.k) * P.ldx : reinterpret_cast<const T *>(P.h) + (long long)place * P.ff;
+        const T *a[N];
 #pragma unroll
-    for (int r = 0; r < N; r++) {
-        const T *W = reinterpret_cast<const T *>(!FIRST ? P.down : r < R ? P.gate : P.up);
-        a[r] = W + ((long long)e * rows + min(row0 + r % R * 16 + c, rows - 1)) * K;
-    }
-    f32x4 acc[N] = {};
-#pragma unroll 4
-    for (int k = w * 32; k < K; k += 128) {
-        const Frag<T> b = load_run<VEC>(x, k + g * 8, K);
+        for (int r = 0; r < N; r++) {
+            const T *W = reinterpret_cast<const T *>(!FIRST ? P.down : r < R ? P.gate : P.up);
+            a[r] = W + ((long long)e * rows + min(row0 + r % R * 16 + c, rows - 1)) * K;
+        }
+        f32x4 acc[N] = {};
+        for (int k = w * 32; k < K; k += 128) {
+            const Frag<T> b = load_run(x, k + g * 8, K);
 #pragma unroll
-        for (int r = 0; r < N; r++) acc[r] = mma(load_run<VEC>(a[r], k + g * 8, K), b, acc[r]);
-    }
+            for (int r = 0; r < N; r++) acc[r] = mma(load_run(a[r], k + g * 8, K), b, acc[r]);
+        }
+        __syncthreads();                                 // (the tile before is read)
 #pragma unroll
-    for (int r = 0; r < N; r++) red[w][r][lane] = acc[r];
-    __syncthreads();
-    if (c >= count) return;
-    for (int r = w; r < R; r += 4) {
+        for (int r = 0; r < N; r++) red[w][r][lane] = acc[r];
+        __syncthreads();
+        if (w >= R || c >= count) continue;
         f32x4 v[M];
 #pragma unroll
-        for (int i = 0; i < M; i++) v[i] = (red[0][r + i * R][lane] + red[1][r + i * R][lane]) + (red[2][r + i * R][lane] + red[3][r + i * R][lane]);
-        const int row = row0 + r * 16 + 4 * g;
+        for (int i = 0; i < M; i++) v[i] = (red[0][w + i * R][lane] + red[1][w + i * R][lane]) + (red[2][w + i * R][lane] + red[3][w + i * R][lane]);
+        const int row = row0 + w * 16 + 4 * g;
         if constexpr (FIRST) put_rows(reinterpret_cast<T *>(P.h) + (long long)place * P.ff, row, P.ff, P.act == NL_ACT_SILU ? activate<true>(v[0], v[1]) : activate<false>(v[0], v[1]));
         else put_rows(P.part + (long long)slot * P.dim, row, P.dim, v[0] * P.weights[slot]);
+    }
+}
+
+// A few tokens: no grouping, no matrix instructions; a row of a matrix is read by a whole wavefront in 16-byte pieces, one row for every slot that
+// asks for it.  First the activations of slot blockIdx.y (h is by slot here), then rows of the sum over token blockIdx.y's slots: a lane keeps its share
+// of all of them, one sum over the wavefront at the end.
+template <typename T> struct Piece { static constexpr int N = 16 / (int)sizeof(T); T v[N]; };
+template <typename T> __device__ __forceinline__ Piece<T> load_piece(const T *p) {
+    Piece<T> r;
+    *reinterpret_cast<f32x4 *>(r.v) = *reinterpret_cast<const f32x4 *>(p);
+    return r;
+}
+template <typename T> __device__ __forceinline__ float dot_piece(const Piece<T> &a, const Piece<T> &b, float s) {
+#pragma unroll
+    for (int i = 0; i < Piece<T>::N; i++) s = fmaf((float)a.v[i], (float)b.v[i], s);
+    return s;
+}
+template <typename T>
+__global__ void __launch_bounds__(256) experts_token_first_kernel(ExpertsParams P) {
+    const int lane = threadIdx.x & 63, row = blockIdx.x * 4 + (threadIdx.x >> 6), slot = blockIdx.y, e = P.ids[slot];
+    if (row >= P.ff || e < 0 || e >= P.experts) return;
+    const T *x = reinterpret_cast<const T *>(P.x) + (long long)(slot / P.k) * P.ldx;
+    const long long at = ((long long)e * P.ff + row) * P.dim;
+    const T *a = reinterpret_cast<const T *>(P.gate) + at, *b = reinterpret_cast<const T *>(P.up) + at;
+    float ga = 0.f, ub = 0.f;
+#pragma unroll 4
+    for (int k = lane * Piece<T>::N; k < P.dim; k += 64 * Piece<T>::N) {
+        const Piece<T> xv = load_piece(x + k), av = load_piece(a + k), bv = load_piece(b + k);
+        ga = dot_piece(av, xv, ga);
+        ub = dot_piece(bv, xv, ub);
+    }
+    ga = wave_sum(ga);
+    ub = wave_sum(ub);
+    if (lane == 0) put(reinterpret_cast<T *>(P.h) + (long long)slot * P.ff + row, ga * sigmoid_f32(P.act == NL_ACT_SILU ? ga : gelu_arg(ga)) * ub);
+}
+template <typename T>
+__global__ void __launch_bounds__(256) experts_token_second_kernel(ExpertsParams P) {
+    const int lane = threadIdx.x & 63, row = blockIdx.x * 4 + (threadIdx.x >> 6), t = blockIdx.y;
+    if (row >= P.dim) return;
+    float sum = 0.f;
+#pragma unroll 4
+    for (int j = 0; j < P.k; j++) {
+        const int slot = t * P.k + j, e = P.ids[slot];
+        if (e < 0 || e >= P.experts) continue;
+        const T *h = reinterpret_cast<const T *>(P.h) + (long long)slot * P.ff, *d = reinterpret_cast<const T *>(P.down) + ((long long)e * P.dim + row) * P.ff;
+        float v = 0.f;
+#pragma unroll 4
+        for (int k = lane * Piece<T>::N; k < P.ff; k += 64 * Piece<T>::N) v = dot_piece(load_piece(d + k), load_piece(h + k), v);
+        sum = fmaf(v, P.weights[slot], sum);
+    }
+    sum = wave_sum(sum);
+    if (lane != 0) return;
+    if (P.y) put(reinterpret_cast<T *>(P.y) + (long long)t * P.ldy + row, sum);
+    else P.part[(long long)t * P.dim + row] = sum;
+}
+
+// Prompts: WR x WT wavefronts of RTW row tiles x NTW token tiles each; 128 bytes of every row at a time go through two LDS stages by LDS-DMA.  A
+// 1 KiB piece is 8 rows x 128 bytes, whole lines of the rows as they lie; in LDS the 16-byte run q of row r is at q ^ (r % 8), so that the 16 rows of a
+// fragment are read from all banks.  FIRST: row tiles alternate between gate and up.
+// Workgroups b, b + 8, ... run on one XCD and take a contiguous range of (expert, row block, token tile): both operands of neighbours are in its L2.
+template <typename T, int RTW_, int NTW_, int WR_, int WT_> struct Grouped {
+    static constexpr int RTW = RTW_, NTW = NTW_, WR = WR_, WT = WT_, RT = WR * RTW, NT = WT * NTW, STAGE = (RT + NT) * 2048, LDS = 2 * STAGE, NW = WR * WT, THREADS = 64 * NW,
+                         PW = STAGE / 1024 / NW, BT = NT * 16, KB = 128 / (int)sizeof(T), KK = KB / 32, PER_CU = 163840 / LDS;
+    static_assert(PW * NW * 1024 == STAGE, "pieces");
+};
+__device__ const f32x4 zero_piece = {0.f, 0.f, 0.f, 0.f};
+template <typename T> __device__ __forceinline__ Frag<T> swizzled_frag(const char *tile, int r, int g, int kk);
+template <> __device__ __forceinline__ Frag<bf16> swizzled_frag<bf16>(const char *tile, int r, int g, int kk) {
+    Frag<bf16> f;
+    f.v = *reinterpret_cast<const bf16x8 *>(tile + r * 128 + (((kk * 4 + g) ^ (r & 7)) << 4));
+    return f;
+}
+template <> __device__ __forceinline__ Frag<float> swizzled_frag<float>(const char *tile, int r, int g, int) {
+    Frag<float> f;
+    f.a = *reinterpret_cast<const f32x4 *>(tile + r * 128 + (((2 * g) ^ (r & 7)) << 4));
+    f.b = *reinterpret_cast<const f32x4 *>(tile + r * 128 + (((2 * g + 1) ^ (r & 7)) << 4));
+    return f;
+}
+template <typename T, bool FIRST, typename S>
+__global__ void __launch_bounds__(S::THREADS, S::NW * S::PER_CU / 4) experts_many_kernel(ExpertsParams P) {
+    constexpr int RT = S::RT, STAGE = S::STAGE, NW = S::NW, PW = S::PW, BT = S::BT, KB = S::KB, KK = S::KK, RTW = S::RTW, NTW = S::NTW;
+    constexpr int BR = (FIRST ? RT / 2 : RT) * 16;        // output rows of the workgroup
+    extern __shared__ __align__(16) char lds[];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15, wr = w % S::WR, wt = w / S::WR;
+    const int rows = FIRST ? P.ff : P.dim, K = FIRST ? P.dim : P.ff, nrb = (rows + BR - 1) / BR, nks = (K + KB - 1) / KB;
+    const Groups<BT> groups(P.offs, P.experts);
+    const int all = groups.total() * nrb, per = (all + 7) >> 3, id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= per || id >= all) return;
+    const Group G = groups.find(id / nrb);
+    const int tiles = (G.b - G.a + BT - 1) / BT, local = id - G.before * nrb, rb = local / tiles, first = G.a + (local - rb * tiles) * BT, count = min(BT, G.b - first);
+    auto row_of = [&](int t, int r) -> const T * {       // row r of tile t of a stage
+        if (t < RT) {
+            const T *W = reinterpret_cast<const T *>(!FIRST ? P.down : t & 1 ? P.up : P.gate);
+            return W + ((long long)G.e * rows + min(rb * BR + (FIRST ? t >> 1 : t) * 16 + r, rows - 1)) * K;
+        }
+        const int place = first + min((t - RT) * 16 + r, count - 1);
+        return FIRST ? reinterpret_cast<const T *>(P.x) + (long long)(P.order[place] / P.k) * P.ldx : reinterpret_cast<const T *>(P.h) + (long long)place * P.ff;
+    };
+    const int turn = rb * nks / nrb;                     // (row blocks start at different columns: their rows would else ask the same memory channels)
+    const char *src[PW];
+    const int k0 = ((lane & 7) ^ (lane >> 3)) * (16 / (int)sizeof(T));
+    int there = 0;                                       // pieces with a token or a row of the matrix: the first ones
+#pragma unroll
+    for (int i = 0; i < PW; i++) {
+        const int u = i * NW + w;
+        if ((u >> 1) < RT || ((u >> 1) - RT) * 16 + (u & 1) * 8 < count) there = i + 1;
+        src[i] = reinterpret_cast<const char *>(row_of(u >> 1, (u & 1) * 8 + (lane >> 3)) + k0);
+    }
+    auto issue = [&](int ks, int st) {
+        if ((ks += turn) >= nks) ks -= nks;
+        if ((ks + 1) * KB <= K) {
+#pragma unroll
+            for (int i = 0; i < PW; i++)
+                if (i < there) lds_dma16(src[i] + (long long)ks * 128, lds + st * STAGE + (i * NW + w) * 1024);
+        } else {                                         // (behind the row's end: zeros)
+            const unsigned long long in = ks * KB + k0 < K ? ~0ull : 0, zero = reinterpret_cast<unsigned long long>(&zero_piece) & ~in;
+#pragma unroll
+            for (int i = 0; i < PW; i++)
+                if (i < there) lds_dma16(reinterpret_cast<const char *>((reinterpret_cast<unsigned long long>(src[i] + (long long)ks * 128) & in) | zero), lds + st * STAGE + (i * NW + w) * 1024);
+        }
+    };
+    f32x4 acc[RTW][NTW] = {};
+    Frag<T> fa[KK][RTW], fb[KK][NTW];
+    const bool busy = wt * NTW * 16 < count;             // (wavefronts without a token only bring pieces)
+    auto read = [&](int st, int kk, Frag<T> *a, Frag<T> *b) {
+        const char *base = lds + st * STAGE;
+#pragma unroll
+        for (int t = 0; t < NTW; t++) b[t] = swizzled_frag<T>(base + (RT + wt * NTW + t) * 2048, c, g, kk);
+#pragma unroll
+        for (int r = 0; r < RTW; r++) a[r] = swizzled_frag<T>(base + (wr * RTW + r) * 2048, c, g, kk);
+    };
+    auto multiply = [&](const Frag<T> *a, const Frag<T> *b) {
+#pragma unroll
+        for (int r = 0; r < RTW; r++)
+#pragma unroll
+            for (int t = 0; t < NTW; t++) acc[r][t] = mma(a[r], b[t], acc[r][t]);
+    };
+    // (builtins, not lds_barrier(): the compiler has to know that nothing is on its way from LDS, or it waits for the next fragments before it
+    // multiplies the present ones)
+    auto arrived = [&]() { __builtin_amdgcn_s_waitcnt(0xc07f); };
+    auto next_stage = [&](int s) {                       // to stage s < nks; the one before it is read and filled again
+        vm_wait<0>();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (s + 1 < nks) issue(s + 1, (s + 1) & 1);
+    };
+    issue(0, 0);
+    if (nks > 1) issue(1, 1);
+    if (nks > 1 && there == PW) vm_wait<PW>();
+    else vm_wait<0>();
+    lds_barrier();
+    if (!busy) {
+        for (int s = 1; s < nks; s++) next_stage(s);
+        return;
+    }
+    // 32 columns a step; a step's fragments are read while the step before it is multiplied.  Once every wavefront has read the last of a
+    // stage (the barrier), the stage is filled again.
+    read(0, 0, fa[0], fb[0]);
+    for (int s = 0; s + 1 < nks; s++) {
+        arrived();
+        if constexpr (KK == 2) {
+            read(s & 1, 1, fa[1], fb[1]);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(fa[0], fb[0]);
+            __builtin_amdgcn_sched_barrier(0);
+            arrived();
+        }
+        next_stage(s + 1);
+        if constexpr (KK == 2) {
+            read(~s & 1, 0, fa[0], fb[0]);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(fa[1], fb[1]);
+        } else {
+            multiply(fa[0], fb[0]);
+            read(~s & 1, 0, fa[0], fb[0]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (KK == 2) read((nks - 1) & 1, 1, fa[1], fb[1]);
+    multiply(fa[0], fb[0]);
+    if constexpr (KK == 2) multiply(fa[1], fb[1]);
+#pragma unroll
+    for (int t = 0; t < NTW; t++) {
+        const int at = (wt * NTW + t) * 16 + c, place = first + at;
+        if (at >= count) continue;
+        if constexpr (FIRST) {
+            T *h = reinterpret_cast<T *>(P.h) + (long long)place * P.ff;
+#pragma unroll
+            for (int r = 0; r < RTW; r += 2)
+                put_rows(h, rb * BR + (wr * RTW + r) * 8 + 4 * g, P.ff, P.act == NL_ACT_SILU ? activate<true>(acc[r][t], acc[r + 1][t]) : activate<false>(acc[r][t], acc[r + 1][t]));
+        } else {
+            const int slot = P.order[place];
+            float *o = P.part + (long long)slot * P.dim;
+            const float wgt = P.weights[slot];
+#pragma unroll
+            for (int r = 0; r < RTW; r++) put_rows(o, rb * BR + (wr * RTW + r) * 16 + 4 * g, P.dim, acc[r][t] * wgt);
+        }
     }
 }
 
@@ -309,12 +499,115 @@ template <typename T> __device__ __forceinline__ float close_value(const ClosePa
     if (P.part)
         for (int j = 0; j < P.k; j++) {
             const long long s = (long long)t * P.k + j;
-            const int id = P.ids[s];
+            const int id = P.ids ? P.ids[s] : 0;
             if (id >= 0 && id < P.experts) v += P.part[s * P.dim + k];
         }
     return v;
 }
-// a workgroup per token
+// V consecutive elements as floats
+template <int V> __device__ __forceinline__ void load_vec(const float *p, float *v) {
+    if constexpr (V == 4) *reinterpret_cast<f32x4 *>(v) = *reinterpret_cast<const f32x4 *>(p);
+    else v[0] = *p;
+}
+template <int V> __device__ __forceinline__ void load_vec(const bf16 *p, float *v) {
+    if constexpr (V == 4) {
+        const bf16x4 b = *reinterpret_cast<const bf16x4 *>(p);
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = (float)b[i];
+    } else v[0] = (float)*p;
+}
+template <int V, typename T> __device__ __forceinline__ void store_vec(T *p, const float *v) {
+    if constexpr (V == 4) put4(p, *reinterpret_cast<const f32x4 *>(v));
+    else put(p, v[0]);
+}
+// A workgroup per token, the row in registers: C runs of V elements a thread, read once; everything that the norms do not decide is on its way before
+// the first of them.
+template <typename T, int V, int C>
+__global__ void __launch_bounds__(256) close_rows_kernel(CloseParams P) {
+    __shared__ float red[2][4];
+    const int t = blockIdx.x, tid = threadIdx.x;
+    float v[C][V], x[C][V], g[C][V], p[C][V];
+    auto at = [&](int c) { return (c * 256 + tid) * V; };
+#pragma unroll
+    for (int c = 0; c < C; c++)
+#pragma unroll
+        for (int i = 0; i < V; i++) { v[c][i] = 0.f; x[c][i] = 0.f; g[c][i] = 1.f; p[c][i] = 0.f; }
+    auto total = [&](int i) {
+        float s = 0.f;
+#pragma unroll
+        for (int c = 0; c < C; c++)
+#pragma unroll
+            for (int j = 0; j < V; j++) s = fmaf(v[c][j], v[c][j], s);
+        s = wave_sum(s);
+        if ((tid & 63) == 0) red[i][tid >> 6] = s;
+        __syncthreads();
+        return (red[i][0] + red[i][1]) + (red[i][2] + red[i][3]);
+    };
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+        const int k = at(c);
+        if (k >= P.dim) break;
+        if (P.d) load_vec<V>(reinterpret_cast<const T *>(P.d) + (long long)t * P.ldd + k, v[c]);
+        else if (P.base) load_vec<V>(P.base + (long long)t * P.ldbase + k, v[c]);
+        if (P.x_out) {
+            load_vec<V>(P.x + (long long)t * P.ldx + k, x[c]);
+            if (P.add) {
+                float o[V];
+                load_vec<V>(P.add + (long long)t * P.ldadd + k, o);
+#pragma unroll
+                for (int i = 0; i < V; i++) x[c][i] += o[i];
+            }
+            if (P.gate) load_vec<V>(P.gate + (long long)t * P.ldgate + k, g[c]);
+            if (P.post) {
+                float o[V];
+                load_vec<V>(P.post + k, o);
+#pragma unroll
+                for (int i = 0; i < V; i++) g[c][i] *= o[i];
+            }
+            if (P.h) load_vec<V>(P.pre + k, p[c]);
+        }
+    }
+    if (P.part) {
+#pragma unroll 4
+        for (int j = 0; j < P.k; j++) {                  // (results of slots without an expert are read and left out: the workspace has room for them)
+            const long long s = (long long)t * P.k + j;
+            const int id = P.ids ? P.ids[s] : 0;
+            const bool in = id >= 0 && id < P.experts;
+#pragma unroll
+            for (int c = 0; c < C; c++) {
+                if (at(c) >= P.dim) break;
+                float o[V];
+                load_vec<V>(P.part + s * P.dim + at(c), o);
+#pragma unroll
+                for (int i = 0; i < V; i++) v[c][i] += in ? o[i] : 0.f;
+            }
+        }
+    }
+    if (!P.x_out) {
+#pragma unroll
+        for (int c = 0; c < C; c++)
+            if (at(c) < P.dim) store_vec<V>(reinterpret_cast<T *>(P.y) + (long long)t * P.ldy + at(c), v[c]);
+        return;
+    }
+    const float inv = P.scale * (P.post ? rsqrt_f32(total(0) / (float)P.dim + P.eps) : 1.f);
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+        if (at(c) >= P.dim) break;
+#pragma unroll
+        for (int i = 0; i < V; i++) v[c][i] = fmaf(inv * v[c][i], g[c][i], x[c][i]);
+        store_vec<V>(P.x_out + (long long)t * P.ldxo + at(c), v[c]);
+    }
+    if (!P.h) return;
+    const float ih = rsqrt_f32(total(1) / (float)P.dim + P.eps);
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+        if (at(c) >= P.dim) break;
+#pragma unroll
+        for (int i = 0; i < V; i++) v[c][i] *= ih * p[c][i];
+        store_vec<V>(reinterpret_cast<T *>(P.h) + (long long)t * P.ldh + at(c), v[c]);
+    }
+}
+// rows of any length, which are read again for every step
 template <typename T>
 __global__ void __launch_bounds__(256) close_kernel(CloseParams P) {
     __shared__ float red[2][4];

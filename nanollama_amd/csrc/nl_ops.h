@@ -28,12 +28,13 @@ struct ExpertsParams {
     int *offs, *order;                    // first place of every expert [experts + 1]; place -> slot (token * k + j)
     void *h;                              // [place][ff] activations
     float *part;                          // [slot][dim] weighted results
+    void *y;                              // launch_experts has these
+    long long ldy;
 };
 // bytes of the workspace and where its parts start
 struct ExpertsLayout { size_t offs, order, h, part, bytes; };
 ExpertsLayout experts_layout(int n, int k, int experts, int dim, int ff, int dtype);
-// everything up to the weighted results in `part`; slots whose id is no expert are left as they are
-hipError_t launch_experts(const ExpertsParams &P, int dtype, hipStream_t st);
+void place_experts(ExpertsParams &P, void *workspace, const ExpertsLayout &L);
 
 // the sum of a token's results (part, ids; null: none) and of `base` (null: none) is d:  x_out = x + add + scale gate v, h = norm(x_out) pre
 struct CloseParams {
@@ -42,7 +43,7 @@ struct CloseParams {
     const void *d;                        // rows of the element type, instead of part and base
     long long ldd;
     const float *part;                    // [slot][dim]
-    const int *ids;
+    const int *ids;                       // null: a row of part a token
     int k, experts;
     const float *post, *gate, *pre;
     long long ldgate;
@@ -54,5 +55,7 @@ struct CloseParams {
     float eps, scale;
 };
 hipError_t launch_close(const CloseParams &P, int dtype, hipStream_t st);
+// the experts' products of P's tokens and the close C of their sums (its part, ids, k, experts, n and dim are filled in)
+hipError_t launch_experts(ExpertsParams P, CloseParams C, int dtype, hipStream_t st);
 
 }  // namespace nl

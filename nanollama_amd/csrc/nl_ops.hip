@@ -2,6 +2,7 @@
 #include "nl_experts.h"
 
 #include <climits>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <algorithm>
@@ -18,6 +19,13 @@ hipError_t start(void (*kernel)(F...), dim3 grid, dim3 block, size_t lds, hipStr
     void *at[sizeof...(F)];
     std::apply([&](auto &...a) { int i = 0; ((at[i++] = (void *)&a), ...); }, held);
     return hipLaunchKernel(reinterpret_cast<const void *>(kernel), grid, block, at, lds, st);
+}
+
+// the same with more dynamic LDS than a kernel has by itself (asked for once a device and kernel; the flag is a hint, a second time does no harm)
+template <typename... F, typename... A>
+hipError_t start_lds(void (*kernel)(F...), dim3 grid, dim3 block, size_t lds, hipStream_t st, A... args) {
+    const hipError_t rc = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    return rc != hipSuccess ? rc : start(kernel, grid, block, lds, st, args...);
 }
 
 inline bool on16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -47,27 +55,92 @@ ExpertsLayout experts_layout(int n, int k, int experts, int dim, int ff, int dty
     L.bytes = L.part + up(slots * dim * 4);
     return L;
 }
+void place_experts(ExpertsParams &P, void *workspace, const ExpertsLayout &L) {
+    char *ws = reinterpret_cast<char *>(workspace);
+    P.offs = reinterpret_cast<int *>(ws + L.offs);
+    P.order = reinterpret_cast<int *>(ws + L.order);
+    P.h = ws + L.h;
+    P.part = reinterpret_cast<float *>(ws + L.part);
+}
 
-template <typename T> static hipError_t experts(const ExpertsParams &P, hipStream_t st) {
+// One product of the experts with tiles of S.
+template <typename T, bool FIRST, typename S> static hipError_t grouped(const ExpertsParams &P, hipStream_t st) {
+    const int slots = P.n * P.k, hit = std::min(P.experts, slots), rows = FIRST ? P.ff : P.dim, br = S::RT * (FIRST ? 8 : 16);
+    const long long most = ((hit + (slots - hit) / S::BT) * (long long)((rows + br - 1) / br) + 7) / 8 * 8;
+    if (most > INT_MAX / S::THREADS) return hipErrorInvalidConfiguration;
+    return start_lds(experts_many_kernel<T, FIRST, S>, dim3((unsigned)most), dim3(S::THREADS), S::LDS, st, P);
+}
+// What tiles of S are expected to take, in us: rounds of workgroups over the CUs x (stages + what a workgroup has in front of and behind them).
+template <bool FIRST, typename S> static double grouped_us(const ExpertsParams &P, double stage) {
+    const double slots = (double)P.n * P.k, hit = std::min<double>(P.experts, slots), tiles = std::max(hit, slots / S::BT + hit / 2);
+    const int rows = FIRST ? P.ff : P.dim, K = FIRST ? P.dim : P.ff, br = S::RT * (FIRST ? 8 : 16);
+    return std::ceil(tiles * ((rows + br - 1) / br) / (256 * S::PER_CU)) * (stage * ((K + S::KB - 1) / S::KB) + 5);
+}
+// Which tiles.  bfloat16, rows x tokens 128 x 64 (three workgroups a CU), 128 x 128 (two) or 256 x 256 (one), whichever is expected to be done first;
+// a stage takes 1.05, 1.05 and 1.8 us there.  us measured of a product with gate and up / with down:
+//   64 experts of 1536 x 768, 8 a token, 2047 tokens   150 / 100   125 / 86   139 / 97        512 tokens   77 / 45   75 / 46   87 / 52
+//   8 of 4096 x 11008, 2 a token, 993 tokens           -           549 / 444  567 / 314       256 tokens   297 / 183  312 / 201  329 / 260
+//   8 of 768 x 2048, 2 a token, 1000 tokens            30 / 30     31 / 33    29 / 55
+// 64 x 64 where 128 x 64 has no workgroup for every CU: down of the last at 333 tokens 18.5 instead of 21.4; but 28 instead of 23 at 16 tokens of the first,
+// which has 672.  32 bits: always 64 x 64, bound by the matrix rate (77 tokens to 4 of 16 of 760 x 500: 23 / 16, with 128 x 64 35 / 24, 128 x 128 55 / 38;
+// 1024 tokens of the first 521 / 265, 527 / 267, 596 / 319).
+template <typename T, bool FIRST> static hipError_t grouped_product(const ExpertsParams &P, hipStream_t st) {
+    using Small = Grouped<T, 2, 2, 2, 2>;
+    if constexpr (sizeof(T) == 2) {
+        using Low = Grouped<T, 4, 2, 2, 2>;
+        using Square = Grouped<T, 4, 4, 2, 2>;
+        using Large = Grouped<T, 8, 4, 2, 4>;
+        const double low = grouped_us<FIRST, Low>(P, 1.05), square = grouped_us<FIRST, Square>(P, 1.05);
+        if (grouped_us<FIRST, Large>(P, 1.8) < std::min(low, square)) return grouped<T, FIRST, Large>(P, st);
+        if (square < low) return grouped<T, FIRST, Square>(P, st);
+        const int slots = P.n * P.k, rows = FIRST ? P.ff : P.dim, br = Low::RT * (FIRST ? 8 : 16);
+        if (std::min(P.experts, slots) + slots / Low::BT / 2 > 256 / ((rows + br - 1) / br)) return grouped<T, FIRST, Low>(P, st);
+    }
+    return grouped<T, FIRST, Small>(P, st);
+}
+template <typename T> static hipError_t experts(const ExpertsParams &P, bool &summed, hipStream_t st) {
     const int slots = P.n * P.k;
-    hipError_t rc = start(plan_kernel, dim3(P.experts), dim3(1024), 0, st, P.ids, slots, P.experts, P.offs, P.order);
-    if (rc != hipSuccess) return rc;
     constexpr int W = 16 / (int)sizeof(T);               // elements of a 16-byte piece
     const bool vec = on16(P.x) && on16(P.gate) && on16(P.up) && on16(P.down) && P.ldx % W == 0 && P.dim % W == 0 && P.ff % W == 0;
-    const int hit = std::min(P.experts, slots), tiles = hit + (slots - hit) / 16;
-    constexpr int R = 2;
-    const dim3 g1((P.ff + 16 * R - 1) / (16 * R), tiles), g2((P.dim + 16 * R - 1) / (16 * R), tiles);
-    if (vec) {
-        if ((rc = start(experts_few_kernel<T, true, true, R>, g1, dim3(256), 0, st, P)) != hipSuccess) return rc;
-        return start(experts_few_kernel<T, false, true, R>, g2, dim3(256), 0, st, P);
+    hipError_t rc;
+    // Slot by slot where grouping hardly saves a matrix: one token, or half as many slots as experts (4 tokens to 8 of 64 of 1536 x 768 38 us, grouped 48;
+    // 8 tokens 68 and 60.  2 tokens to 2 of 8 of 4096 x 11008 188 and 240, 4 tokens 349 and 280).
+    summed = vec && (P.n == 1 || 2ll * slots <= P.experts);
+    if (summed) {
+        if ((rc = start(experts_token_first_kernel<T>, dim3((P.ff + 3) / 4, slots), dim3(256), 0, st, P)) != hipSuccess) return rc;
+        return start(experts_token_second_kernel<T>, dim3((P.dim + 3) / 4, P.n), dim3(256), 0, st, P);
     }
-    if ((rc = start(experts_few_kernel<T, true, false, R>, g1, dim3(256), 0, st, P)) != hipSuccess) return rc;
-    return start(experts_few_kernel<T, false, false, R>, g2, dim3(256), 0, st, P);
+    if ((rc = start(plan_kernel, dim3(P.experts), dim3(1024), 0, st, P.ids, slots, P.experts, P.offs, P.order)) != hipSuccess) return rc;
+    if (vec) {
+        if ((rc = grouped_product<T, true>(P, st)) != hipSuccess) return rc;
+        return grouped_product<T, false>(P, st);
+    }
+    const int hit = std::min(P.experts, slots), tiles = std::min(hit + (slots - hit) / 16, 65535);
+    if ((rc = start(experts_any_kernel<T, true>, dim3((P.ff + 31) / 32, tiles), dim3(256), 0, st, P)) != hipSuccess) return rc;
+    return start(experts_any_kernel<T, false>, dim3((P.dim + 31) / 32, tiles), dim3(256), 0, st, P);
 }
-hipError_t launch_experts(const ExpertsParams &P, int dtype, hipStream_t st) { return dtype == NL_DTYPE_F32 ? experts<float>(P, st) : experts<bf16>(P, st); }
 
-hipError_t launch_close(const CloseParams &P, int dtype, hipStream_t st) {
-    return dtype == NL_DTYPE_F32 ? start(close_kernel<float>, dim3(P.n), dim3(256), 0, st, P) : start(close_kernel<bf16>, dim3(P.n), dim3(256), 0, st, P);
+template <typename T> static hipError_t close(const CloseParams &P, hipStream_t st) {
+    auto four = [](const void *p, long long ld, size_t size) { return (reinterpret_cast<uintptr_t>(p) & (4 * size - 1)) == 0 && ld % 4 == 0; };
+    const bool v4 = P.dim % 4 == 0 && four(P.x, P.ldx, 4) && four(P.add, P.ldadd, 4) && four(P.base, P.ldbase, 4) && four(P.d, P.ldd, sizeof(T)) && four(P.part, 0, 4) &&
+                    four(P.post, 0, 4) && four(P.gate, P.ldgate, 4) && four(P.pre, 0, 4) && four(P.x_out, P.ldxo, 4) && four(P.h, P.ldh, sizeof(T)) && four(P.y, P.ldy, sizeof(T));
+    const dim3 grid(P.n), block(256);
+    if (v4 && P.dim <= 1024) return start(close_rows_kernel<T, 4, 1>, grid, block, 0, st, P);
+    if (v4 && P.dim <= 2048) return start(close_rows_kernel<T, 4, 2>, grid, block, 0, st, P);
+    if (v4 && P.dim <= 4096) return start(close_rows_kernel<T, 4, 4>, grid, block, 0, st, P);
+    if (P.dim <= 1024) return start(close_rows_kernel<T, 1, 4>, grid, block, 0, st, P);
+    if (P.dim <= 4096) return start(close_rows_kernel<T, 1, 16>, grid, block, 0, st, P);
+    return start(close_kernel<T>, grid, block, 0, st, P);
+}
+hipError_t launch_close(const CloseParams &P, int dtype, hipStream_t st) { return dtype == NL_DTYPE_F32 ? close<float>(P, st) : close<bf16>(P, st); }
+hipError_t launch_experts(ExpertsParams P, CloseParams C, int dtype, hipStream_t st) {
+    C.part = P.part; C.ids = P.ids; C.k = P.k; C.experts = P.experts; C.n = P.n; C.dim = P.dim;
+    if (!C.x_out && !C.base) { P.y = C.y; P.ldy = C.ldy; }
+    bool summed = false;
+    const hipError_t rc = dtype == NL_DTYPE_F32 ? experts<float>(P, summed, st) : experts<bf16>(P, summed, st);
+    if (rc != hipSuccess || (summed && P.y)) return rc;
+    if (summed) { C.ids = nullptr; C.k = 1; }
+    return launch_close(C, dtype, st);
 }
 
 }  // namespace nl
@@ -158,17 +231,13 @@ int nl_op_experts(int device, void *stream, const nl_experts_desc *d, int n, con
     const ExpertsLayout L = experts_layout(n, d->per_token, d->experts, d->dim, d->ff, d->dtype);
     if (workspace_bytes < L.bytes) return fail(NL_ERR_INVALID, "experts: workspace of %llu bytes, %llu are needed", (unsigned long long)workspace_bytes, (unsigned long long)L.bytes);
     if (!on16(workspace)) return fail(NL_ERR_INVALID, "experts: workspace is not on a 16-byte boundary");
-    char *ws = reinterpret_cast<char *>(workspace);
     ExpertsParams P{};
     P.x = x; P.gate = gate; P.up = up; P.down = down; P.ldx = ldx; P.ids = ids; P.weights = weights; P.n = n; P.k = d->per_token; P.experts = d->experts;
     P.dim = d->dim; P.ff = d->ff; P.act = d->act;
-    P.offs = reinterpret_cast<int *>(ws + L.offs); P.order = reinterpret_cast<int *>(ws + L.order); P.h = ws + L.h; P.part = reinterpret_cast<float *>(ws + L.part);
+    place_experts(P, workspace, L);
     CloseParams C{};
-    C.part = P.part; C.ids = ids; C.k = P.k; C.experts = P.experts; C.y = y; C.ldy = ldy; C.n = n; C.dim = d->dim;
-    return on_device("experts", device, stream, [&](hipStream_t st) {
-        const hipError_t rc = launch_experts(P, d->dtype, st);
-        return rc != hipSuccess ? rc : launch_close(C, d->dtype, st);
-    });
+    C.y = y; C.ldy = ldy;
+    return on_device("experts", device, stream, [&](hipStream_t st) { return launch_experts(P, C, d->dtype, st); });
 }
 
 int nl_op_residual_norm(int device, void *stream, const nl_residual_norm_desc *d, int n, const float *x, int64_t ldx, const void *b, int64_t ldb, const float *post,
