@@ -5,7 +5,7 @@
  *   nl_op_experts         y = sum over a token's experts of weight * down(act(gate x) * up x), the tokens grouped by expert
  *   nl_op_residual_norm   what closes a block: norm behind it, gate, residual scale, norm in front of the next
  *
- * The layer-stack models call the same kernels for layers that nl_stack_experts has given experts (below).
+ * Layer-stack models call the same kernels for layers that nl_stack_experts (below) has given experts.
  *
  * Conventions.  Pointers are device memory of `device` that the caller owns, unless a comment says otherwise; nothing is kept behind a
  * return, and no call allocates, synchronises or copies to the host: work is queued on `stream` (a hipStream_t of `device`, NULL: its
@@ -71,6 +71,19 @@ typedef struct {
 NL_API int nl_op_residual_norm(int device, void *stream, const nl_residual_norm_desc *d, int n, const float *x, int64_t ldx, const void *b,
                                int64_t ldb, const float *post, const float *gate, int64_t ldgate, const float *pre, float *x_out,
                                int64_t ldxo, void *h, int64_t ldh);
+
+/* Experts as the feed-forward of a layer of a model that nl_create_stack made, before its tensors are uploaded:
+ *     h = norm2 x;   x += experts(h), the choice by ff.router h;   with post_norm x += norm2_post(experts(h))
+ * The layer's nl_layer_desc has ff == 0.  Tensors: norm2 (and norm2_post) as for a feed-forward, and
+ *     layers.N.ff.router                       [experts, dim],  ff.router_bias [experts] with bias (sigmoid scores only, joins the choice alone)
+ *     layers.N.ff.experts.gate / up            [experts * ff, dim], expert behind expert
+ *     layers.N.ff.experts.down                 [experts * dim, ff] */
+typedef struct {
+    int32_t experts, per_token, ff, act;        /* ff: width of an expert; act: NL_ACT_* */
+    int32_t score, renorm, bias;                /* as in nl_route_desc */
+    float scale;
+} nl_stack_experts_desc;
+NL_API int nl_stack_experts(nl_handle h, int layer, const nl_stack_experts_desc *d);
 
 #ifdef __cplusplus
 }

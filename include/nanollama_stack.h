@@ -12,7 +12,7 @@
  * A layer is up to three residual branches' worth of description:
  *     x += mix_scale terms of { attention(norm1 x), linear_attention(norm1 x) }        (either may be absent), or
  *     x += latent_attention(norm1 x)
- *     x += down(act(gate(norm2 x)) * up(norm2 x))                                      (absent when ff == 0)
+ *     x += down(act(gate(norm2 x)) * up(norm2 x))                                      (absent when ff == 0; experts instead: nanollama_ops.h)
  * With post_norm every sublayer's result goes through a norm of its own before it is added: x += norm1_post(mixer(norm1 x)), ....
  * Norms are x / sqrt(mean(x^2) + eps) * (1 + w), or * w with plain_norm.  Tensor names for nl_upload_tensor (matrices [out, in]):
  *     embed                                    [vocab, dim]     token table; also the output matrix unless untied

@@ -66,6 +66,11 @@ class NlRouteDesc(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("experts", "per_token", "score", "renorm")] + [("scale", C.c_float)]
 
 
+class NlStackExpertsDesc(C.Structure):
+    """nl_stack_experts_desc: experts as a layer's feed-forward."""
+    _fields_ = [(n, C.c_int32) for n in ("experts", "per_token", "ff", "act", "score", "renorm", "bias")] + [("scale", C.c_float)]
+
+
 class NlExpertsDesc(C.Structure):
     """nl_experts_desc: sizes of a feed-forward of experts."""
     _fields_ = [(n, C.c_int32) for n in ("experts", "per_token", "dim", "ff", "act", "dtype")]
@@ -153,7 +158,7 @@ STACK_EXPORTS = ["nl_build_info", "nl_abi_version", "nl_device_count", "nl_creat
                  "nl_last_error", "nl_reset", "nl_forward", "nl_forward_argmax", "nl_decode_greedy", "nl_prefill", "nl_forward_batch",
                  "nl_get_config", "nl_synchronize", "nl_timer_start", "nl_timer_stop", "nl_memory_usage", "nl_debug_read",
                  "nl_sample_decode", "nl_host_logits", "nl_step", "nl_trace_layers", "nl_op_route", "nl_op_experts",
-                 "nl_op_experts_workspace", "nl_op_residual_norm"]
+                 "nl_op_experts_workspace", "nl_op_residual_norm", "nl_stack_experts"]
 
 _vp, _i32, _fp, _ip = C.c_void_p, C.c_int, C.POINTER(C.c_float), C.POINTER(C.c_int)
 
@@ -237,6 +242,7 @@ def stack_lib():
         L.nl_create_stack.argtypes = [C.POINTER(NlStackConfig), C.POINTER(NlLayerDesc), C.POINTER(_vp)]
         L.nl_step.argtypes = [_vp, _i32, _ip, _ip, _ip, _ip, _i32, _ip, _fp, _ip]
         L.nl_trace_layers.argtypes = [_vp, _i32]
+        L.nl_stack_experts.argtypes = [_vp, _i32, C.POINTER(NlStackExpertsDesc)]
         L.nl_op_route.argtypes = [_i32, _vp, C.POINTER(NlRouteDesc), _i32, _vp, C.c_int64, _vp, _vp, _vp]
         L.nl_op_experts.argtypes = [_i32, _vp, C.POINTER(NlExpertsDesc), _i32, _vp, C.c_int64] + [_vp] * 6 + [C.c_int64, _vp, C.c_uint64]
         L.nl_op_experts_workspace.argtypes = [C.POINTER(NlExpertsDesc), _i32]

@@ -63,6 +63,13 @@ __global__ void widen_kernel(const void *src, int src_f32, long long n, float ad
                           : __uint_as_float((unsigned)reinterpret_cast<const unsigned short *>(src)[i] << 16)) + add;
 }
 
+// row-major in the element type
+template <typename T>
+__global__ void plain_kernel(const void *src, int src_f32, long long n, T *dst) {
+    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x)
+        put(dst + i, src_f32 ? reinterpret_cast<const float *>(src)[i] : __uint_as_float((unsigned)reinterpret_cast<const unsigned short *>(src)[i] << 16));
+}
+
 // ---------------------------------------------------- embedding, norm ---
 
 struct LookupParams {

@@ -7,6 +7,7 @@
 //     lookup -> per layer run { [norm +] projections -> mixers -> output matrix + residual -> [norm +] gate | up -> down + residual }
 //            -> [norm +] logits
 //
+// (a layer of experts instead: output matrix -> residual and norm -> [norm +] router -> choice -> experts -> sum and residual, nl_ops.h)
 // with the norm inside the product's launch for a handful of tokens and in a launch of its own otherwise.  A latent-attention mixer is
 // two more products (nl_latent.h).  Where a model has norms behind its sublayers a product leaves its plain result, and the next launch
 // that norms the residual stream adds it on the way, from one stream buffer to the other.  Layers of a loop are run
@@ -49,6 +50,10 @@ struct Layer {
     Mat uq, uk, ukt, uv;         // latent attention: queries; keys and values from the latent; its transpose, a group of rows per head
     float *norm1p = nullptr, *norm2p = nullptr, *dqnorm = nullptr, *kvnorm = nullptr, *sink = nullptr, *rope = nullptr;
     float *gateb = nullptr, *upb = nullptr, *downb = nullptr;
+    nl_stack_experts_desc x{};   // experts > 0: a feed-forward of experts, rows as they come
+    Mat router;
+    float *routerb = nullptr;
+    void *xgate = nullptr, *xup = nullptr, *xdown = nullptr;
     int tdq = 0, tdkv = 0, tg = -1, dimp = 0, rotp = 0, vdp = 0, kvt = 0;   // latent: projection rows, padded sizes, cache tiles of c (nks: all)
     float *norm1 = nullptr, *norm2 = nullptr, *qnorm = nullptr, *knorm = nullptr, *a2 = nullptr, *a2b = nullptr, *lnorm = nullptr, *slope = nullptr;
     int aq = 0, ak = 0, av = 0, ag = -1, lq = 0, lk = 0, lv = 0, lg = 0, la1 = 0;   // rows of the projection matrix
@@ -102,6 +107,10 @@ struct nl_engine {
     int kv_slots = 0;
     bool latent = false;
     void *h = nullptr, *y = nullptr, *act = nullptr, *q = nullptr;
+    // experts: normed rows, logits, choices, weights, workspace
+    void *hrow = nullptr, *xws = nullptr;
+    float *rlogits = nullptr, *rweights = nullptr;
+    int *rids = nullptr;
     float *ldec = nullptr, *inc = nullptr, *totlog = nullptr, *part = nullptr;
     unsigned *arrived = nullptr;
     float *amax_val = nullptr;   // one token's logits: the largest of every 16 rows (the argmax reads these)
@@ -171,6 +180,7 @@ struct Dest {                    // where a tensor goes
     float *vec = nullptr;        // ... or plain float, plus `add`, transposed if asked for
     bool transpose = false;
     float add = 0.f;
+    void *plain = nullptr;       // ... or rows as they are, in the element type
     // a place per source row instead (pack_mapped_kernel), in one or two matrices
     std::vector<int> rbase[2], kbase[2];
     Mat *mapped[2] = {nullptr, nullptr};
@@ -261,6 +271,17 @@ bool find_dest(nl_engine *e, const char *name, Dest &d) {
         if (f == "lin.norm") return vec(L.lnorm, 1, G.vdim, 0.f);
         if (f == "lin.o") { d.mat = &L.out; d.k0 = L.y_lin; d.rows = D; d.cols = G.heads * G.vdim; return true; }
     }
+    if (L.x.experts) {
+        const long long E = L.x.experts, F = L.x.ff;
+        auto plain = [&](void *p, long long rows, long long cols) { d.plain = p; d.rows = rows; d.cols = cols; return true; };
+        if (f == "norm2") return vec(L.norm2, 1, D, unit);
+        if (f == "norm2_post" && e->c.post_norm) return vec(L.norm2p, 1, D, unit);
+        if (f == "ff.router") { d.mat = &L.router; d.rows = E; d.cols = D; return true; }
+        if (f == "ff.router_bias" && L.x.bias) return vec(L.routerb, 1, E, 0.f);
+        if (f == "ff.experts.gate") return plain(L.xgate, E * F, D);
+        if (f == "ff.experts.up") return plain(L.xup, E * F, D);
+        if (f == "ff.experts.down") return plain(L.xdown, E * D, F);
+    }
     if (L.d.ff) {
         if (f == "norm2") return vec(L.norm2, 1, D, unit);
         if (f == "norm2_post" && e->c.post_norm) return vec(L.norm2p, 1, D, unit);
@@ -300,6 +321,12 @@ std::vector<std::string> wanted_tensors(const nl_engine *e) {
             add({"norm2", "ff.gate", "ff.up", "ff.down"});
             if (e->c.post_norm) add({"norm2_post"});
             if (d.ff_bias) add({"ff.gate_bias", "ff.up_bias", "ff.down_bias"});
+        }
+        const nl_stack_experts_desc &x = e->layers[i].x;
+        if (x.experts) {
+            add({"norm2", "ff.router", "ff.experts.gate", "ff.experts.up", "ff.experts.down"});
+            if (e->c.post_norm) add({"norm2_post"});
+            if (x.bias) add({"ff.router_bias"});
         }
     }
     return w;
@@ -513,6 +540,37 @@ hipError_t latent_mixer(nl_engine *e, const StepIn &s, const Run &R, const Layer
     return hipSuccess;
 }
 
+// from the mixer's result to the stream behind the experts; behind: a further addend or null
+template <typename T>
+hipError_t experts_sublayer(nl_engine *e, const Layer &L, int n, const float *behind) {
+    const hipStream_t st = e->stream;
+    const int D = e->c.dim, dtype = e->c.dtype;
+    const nl_stack_experts_desc &x = L.x;
+    hipError_t rc;
+    MatParams O = product_params(e, L.out, e->y, n);
+    O.out = e->delta; O.ldo = D;
+    e->folded = false;
+    if ((rc = launch_product<T, ST_F32>(O, st))) return rc;
+    CloseParams M{};
+    M.x = M.x_out = e->xcur; M.ldx = M.ldxo = D; M.base = e->delta; M.ldbase = D; M.post = L.norm1p; M.pre = L.norm2; M.h = e->hrow; M.ldh = D;
+    M.n = n; M.dim = D; M.eps = e->c.eps; M.scale = 1.f;
+    if ((rc = launch_close(M, dtype, st))) return rc;
+    MatParams J = product_params(e, L.router, nullptr, n);
+    J.out = e->rlogits; J.ldo = L.router.nrt * 16;
+    if ((rc = normed_product<T, ST_F32>(e, J, L.norm2))) return rc;
+    RouteParams P{};
+    P.logits = e->rlogits; P.ld = J.ldo; P.bias = L.routerb; P.n = n; P.experts = x.experts; P.k = x.per_token; P.sigmoid = x.score == NL_SCORE_SIGMOID;
+    P.renorm = x.renorm != 0; P.scale = x.scale; P.ids = e->rids; P.weights = e->rweights;
+    if ((rc = launch_route(P, st))) return rc;
+    ExpertsParams X{};
+    X.x = e->hrow; X.ldx = D; X.gate = L.xgate; X.up = L.xup; X.down = L.xdown; X.ids = e->rids; X.weights = e->rweights; X.n = n; X.k = x.per_token;
+    X.experts = x.experts; X.dim = D; X.ff = x.ff; X.act = x.act;
+    place_experts(X, e->xws, experts_layout(n, x.per_token, x.experts, D, x.ff, dtype));
+    CloseParams C{};
+    C.x = C.x_out = e->xcur; C.ldx = C.ldxo = D; C.add = behind; C.ldadd = D; C.post = L.norm2p; C.eps = e->c.eps; C.scale = 1.f;
+    return launch_experts(X, C, dtype, st);
+}
+
 template <typename T>
 hipError_t launch_sequence(nl_engine *e, const StepIn &s) {
     const hipStream_t st = e->stream;
@@ -569,7 +627,9 @@ hipError_t launch_sequence(nl_engine *e, const StepIn &s) {
             if (A.heads && ((rc = launch_win_prep<T>(W, s.n, st)) || (rc = launch_win_attn<T>(W, s.ntiles, st)))) return rc;
             if (G.heads && (rc = launch_gla<T>(N, s.nsubs, s.nsegs, s.nruns, s.longest, st))) return rc;
         }
-        if ((rc = residual_product<T>(e, L.out, e->y, s.n, nullptr, L.norm1p, L.d.ff ? nullptr : behind, L.d.ff ? L.norm2 : next,
+        if (L.x.experts) {
+            if ((rc = experts_sublayer<T>(e, L, s.n, behind))) return rc;
+        } else if ((rc = residual_product<T>(e, L.out, e->y, s.n, nullptr, L.norm1p, L.d.ff ? nullptr : behind, L.d.ff ? L.norm2 : next,
                                       L.d.ff && L.d.latent.heads ? &L.gateup : nullptr))) return rc;
         if (L.d.ff) {
             MatParams F = product_params(e, L.gateup, nullptr, s.n);
@@ -944,6 +1004,28 @@ int nl_create_stack(const nl_stack_config *cfg, const nl_layer_desc *ld, nl_hand
     return NL_OK;
 }
 
+int nl_stack_experts(nl_handle e, int layer, const nl_stack_experts_desc *d) {
+    if (!e || !d) return NL_ERR_INVALID;
+    if (e->finalized) return e->fail(NL_ERR_STATE, "nl_stack_experts after nl_finalize");
+    if (layer < 0 || layer >= (int)e->layers.size()) return e->fail(NL_ERR_INVALID, "layer %d out of range", layer);
+    Layer &L = e->layers[layer];
+    if (L.x.experts) return e->fail(NL_ERR_STATE, "layer %d has experts already", layer);
+    if (L.d.ff) return e->fail(NL_ERR_UNSUPPORTED, "layer %d: experts beside a feed-forward", layer);
+    if (d->experts < 1 || d->experts > NL_MAX_EXPERTS || d->per_token < 1 || d->per_token > NL_MAX_PER_TOKEN || d->per_token > d->experts)
+        return e->fail(NL_ERR_INVALID, "layer %d: %d of %d experts a token (1 to %d of 1 to %d)", layer, d->per_token, d->experts, NL_MAX_PER_TOKEN, NL_MAX_EXPERTS);
+    if (d->ff < 1 || d->ff > 1 << 20 || e->c.dim > 1 << 20 || (d->act != NL_ACT_SILU && d->act != NL_ACT_GELU_TANH)) return e->fail(NL_ERR_INVALID, "layer %d: width or activation of the experts", layer);
+    if ((d->score != NL_SCORE_SOFTMAX && d->score != NL_SCORE_SIGMOID) || !(d->scale - d->scale == 0.f)) return e->fail(NL_ERR_INVALID, "layer %d: scores of the experts", layer);
+    if (d->bias && d->score != NL_SCORE_SIGMOID) return e->fail(NL_ERR_UNSUPPORTED, "layer %d: a bias goes with sigmoid scores", layer);
+    HIPCK(e, hipSetDevice(e->c.device));
+    const size_t one = (size_t)d->experts * d->ff * e->c.dim * e->esize();
+    size_t &bw = e->bytes_weights;
+    int rc;
+    if ((rc = mat_alloc(e, L.router, d->experts, e->c.dim)) || (rc = dev_alloc(e, L.norm2, (size_t)e->c.dim * 4, bw)) || (rc = dev_alloc(e, L.xgate, one, bw)) ||
+        (rc = dev_alloc(e, L.xup, one, bw)) || (rc = dev_alloc(e, L.xdown, one, bw)) || (d->bias && (rc = dev_alloc(e, L.routerb, (size_t)d->experts * 4, bw)))) return rc;
+    L.x = *d;
+    return NL_OK;
+}
+
 int nl_get_config(nl_handle h, nl_config *out) {
     if (!h || !out) return NL_ERR_INVALID;
     *out = h->cfg;
@@ -986,7 +1068,9 @@ int nl_upload_tensor(nl_handle e, const char *name, uint32_t type, const void *d
         }
         (void)hipFree(maps);
         HIPCK(e, s);
-    } else if (d.vec) hipLaunchKernelGGL(widen_kernel, dim3(grid), dim3(256), 0, e->stream, e->stage, f32, n, d.add, d.vec, d.transpose ? (int)d.cols : 1);
+    } else if (d.plain && e->f32()) hipLaunchKernelGGL(plain_kernel<float>, dim3(grid), dim3(256), 0, e->stream, e->stage, f32, n, reinterpret_cast<float *>(d.plain));
+    else if (d.plain) hipLaunchKernelGGL(plain_kernel<bf16>, dim3(grid), dim3(256), 0, e->stream, e->stage, f32, n, reinterpret_cast<bf16 *>(d.plain));
+    else if (d.vec) hipLaunchKernelGGL(widen_kernel, dim3(grid), dim3(256), 0, e->stream, e->stage, f32, n, d.add, d.vec, d.transpose ? (int)d.cols : 1);
     else if (e->f32()) hipLaunchKernelGGL(pack_operand_kernel<float>, dim3(grid), dim3(256), 0, e->stream, e->stage, f32, d.rows, d.cols, reinterpret_cast<float *>(d.mat->w), d.mat->nks, d.row0, d.k0, d.tstride, d.toff);
     else hipLaunchKernelGGL(pack_operand_kernel<bf16>, dim3(grid), dim3(256), 0, e->stream, e->stage, f32, d.rows, d.cols, reinterpret_cast<bf16 *>(d.mat->w), d.mat->nks, d.row0, d.k0, d.tstride, d.toff);
     HIPCK(e, hipGetLastError());
@@ -1007,7 +1091,10 @@ int nl_finalize(nl_handle e) {
     {   // what a decode step reads: everything but an untied lookup table and the expanded keys' matrix, which prompts use
         auto bytes = [&](const Mat &m) { return m.w ? (size_t)m.nrt * m.nks * OPT * es : 0; };
         size_t read = e->bytes_weights - (e->c.untied ? bytes(e->embed) : 0);
-        for (const Layer &L : e->layers) read -= bytes(L.uk);
+        for (const Layer &L : e->layers) {
+            read -= bytes(L.uk);
+            if (L.x.experts) read -= (size_t)3 * (L.x.experts - L.x.per_token) * L.x.ff * e->c.dim * es;      // (one token's)
+        }
         const char *knob = getenv("NL_STACK_AHEAD");     // knob (tests): 0 never, else always
         e->read_ahead = knob ? atoi(knob) != 0 : read > AHEAD_WEIGHTS;
     }
@@ -1015,6 +1102,7 @@ int nl_finalize(nl_handle e) {
     const int cap = e->cap, few = std::min(std::max(S, 1), FEW_MAX_TOKENS);
     e->lm_cap = std::max(FEW_MAX_TOKENS, std::min(cap, 256));
     int ldmax = 0, yk = 0, ak = 0, hk = e->nksd;
+    size_t xws = 0, xld = 0, xk = 0;
     size_t xq = 0, ek = 0, ev = 0, lpart = 0, lml = 0;
     std::map<std::tuple<int, double, double, double, double, double>, float *> ropes;
     // scratch for expanded keys: the longest sequence, or whole prompts that fill a launch sequence
@@ -1025,6 +1113,10 @@ int nl_finalize(nl_handle e) {
         const nl_attn_desc &A = L.d.attn;
         const nl_linattn_desc &G = L.d.lin;
         ldmax = std::max(ldmax, L.proj.rows); yk = std::max(yk, L.out.nks); ak = std::max(ak, L.d.ff ? L.down.nks : 0);
+        if (L.x.experts) {
+            xws = std::max(xws, experts_layout(cap, L.x.per_token, L.x.experts, D, L.x.ff, e->c.dtype).bytes);
+            xld = std::max(xld, (size_t)L.router.nrt * 16); xk = std::max(xk, (size_t)L.x.per_token);
+        }
         if (A.heads) {
             // the ring: every position while they fit, else what the window needs beside the tokens one launch sequence adds
             const long long whole = up(e->c.seq_len, 64), ring = A.window > 0 ? (long long)up(A.window - 1 + cap, 64) : whole;
@@ -1074,7 +1166,9 @@ int nl_finalize(nl_handle e) {
         (rc = dev_alloc(e, e->proj, (size_t)cap * ldmax * 4, bs)) || (rc = dev_alloc(e, e->logits, (size_t)e->lm_cap * e->c.vocab * 4, bs)) ||
         (rc = dev_alloc(e, e->h, std::max(tt, (size_t)up(e->lm_cap, 128) / 16) * hk * OPT * es, bs)) || (rc = dev_alloc(e, e->fss, (size_t)FEW_MAX_TOKENS * 2 * e->nksd * sizeof(float), bs)) || (rc = dev_alloc(e, e->y, tt * yk * OPT * es, bs)) ||
         (ak && (rc = dev_alloc(e, e->act, tt * ak * OPT * es, bs))) || (qrow && (rc = dev_alloc(e, e->q, std::max((size_t)cap * qrow, qfew) * es, bs))) ||
-        (e->c.post_norm && ((rc = dev_alloc(e, e->x2, (size_t)cap * D * 4, bs)) || (rc = dev_alloc(e, e->delta, (size_t)cap * D * 4, bs)))) ||
+        (e->c.post_norm && (rc = dev_alloc(e, e->x2, (size_t)cap * D * 4, bs))) || ((e->c.post_norm || xk) && (rc = dev_alloc(e, e->delta, (size_t)cap * D * 4, bs))) ||
+        (xk && ((rc = dev_alloc(e, e->hrow, (size_t)cap * D * es, bs)) || (rc = dev_alloc(e, e->rlogits, (size_t)cap * xld * 4, bs)) ||
+                (rc = dev_alloc(e, e->rids, (size_t)cap * xk * 4, bs)) || (rc = dev_alloc(e, e->rweights, (size_t)cap * xk * 4, bs)) || (rc = dev_alloc(e, e->xws, xws, bs)))) ||
         (e->latent && ((rc = dev_alloc(e, e->xq, xq * es, bs)) || (rc = dev_alloc(e, e->ek, ek * es, bs)) || (rc = dev_alloc(e, e->ev, ev * es, bs)) ||
                        (rc = dev_alloc(e, e->lpart, lpart * 4, bs)) || (rc = dev_alloc(e, e->lml, lml * 4, bs)))) ||
         (ldec && ((rc = dev_alloc(e, e->ldec, ldec * 4, bs)) || (rc = dev_alloc(e, e->inc, inc * 4, bs)) || (rc = dev_alloc(e, e->totlog, tot * 4, bs)))) ||

@@ -1,10 +1,11 @@
 """Ganidra: gated linear attention layers ("gla") and layers whose mixer runs windowed softmax attention and gated linear attention
-side by side ("parallel"), an optional gated feed-forward per layer, a range of layers that is run several times, tied output."""
+side by side ("parallel"), an optional gated feed-forward per layer, dense or of experts, a range of layers that is run several times, tied output."""
 from __future__ import annotations
 
 from typing import Callable, Tuple
 
 from ..stack import Attention, LinearAttention, StackLayer, StackSpec
+from .experts import routed_experts
 
 _LIN = {"q": "q", "k": "k", "v": "v", "g": "g", "o": "o", "a1": "a1", "a2": "a2", "a2_bias": "a2.b", "norm": "norm"}
 _ATTN = {"q": "q", "k": "k", "v": "v", "g": "g", "o": "o", "q_norm": "q.norm", "k_norm": "k.norm"}
@@ -36,11 +37,14 @@ def ganidra_spec(cfg: dict, shape: Callable[[str], Tuple[int, ...]]) -> StackSpe
         else:
             raise ValueError(f"layer {i}: unknown mixer type {kind!r}")
         if mlp is not None:
-            if mlp["kind"] != "dense":
+            if mlp["kind"] not in ("dense", "routed"):
                 raise ValueError(f"layer {i}: unknown feed-forward kind {mlp['kind']!r}")
-            layer.ff = mlp["ff"]
             tensors[f"layers.{i}.norm2"] = f"l{i}.norm2"
-            tensors.update({f"layers.{i}.ff.{k}": f"l{i}.mlp.{k}" for k in ("gate", "up", "down")})
+            if mlp["kind"] == "routed":
+                layer.experts = routed_experts(i, mlp, "gelu_tanh", tensors)
+            else:
+                layer.ff = mlp["ff"]
+                tensors.update({f"layers.{i}.ff.{k}": f"l{i}.mlp.{k}" for k in ("gate", "up", "down")})
         layers.append(layer)
     loop = cfg.get("loop")
     return StackSpec("Ganidra", cfg["vocab"], cfg["width"], layers, cfg["norm"]["eps"], cfg["embedding"]["scale"],

@@ -1,11 +1,12 @@
 """Pabalix: latent attention in every layer (three kinds: rotary pairs half a vector apart with YaRN, adjacent pairs where a layer may
 attend an earlier layer's latents, and the first kind with a sink and a gate per head), norms in front of and behind every sublayer, an
-optional silu feed-forward with biases, an output matrix of its own."""
+optional silu feed-forward with biases or of experts, an output matrix of its own."""
 from __future__ import annotations
 
 from typing import Callable, Tuple
 
 from ..stack import LatentAttention, StackLayer, StackSpec, Yarn
+from .experts import routed_experts
 
 # type of a mixer -> (adjacent dimensions are a rotary pair, sink and gate per head)
 KINDS = {"latent_attention": (False, False), "latent_attention_2": (True, False), "latent_attention_3": (False, True)}
@@ -32,11 +33,14 @@ def pabalix_spec(cfg: dict, shape: Callable[[str], Tuple[int, ...]]) -> StackSpe
         tensors.update({f"layers.{i}.latent.{k}": f"l{i}.mix.{v}" for k, v in names.items()})
         tensors.update({f"layers.{i}.norm1": f"l{i}.norm1", f"layers.{i}.norm1_post": f"l{i}.norm1b"})
         if mlp is not None:
-            if mlp["kind"] != "dense":
+            if mlp["kind"] not in ("dense", "routed"):
                 raise ValueError(f"layer {i}: unknown feed-forward kind {mlp['kind']!r}")
-            layer.ff, layer.ff_act, layer.ff_bias = mlp["ff"], "silu", True
             tensors.update({f"layers.{i}.norm2": f"l{i}.norm2", f"layers.{i}.norm2_post": f"l{i}.norm2b"})
-            for k in ("gate", "up", "down"):
-                tensors.update({f"layers.{i}.ff.{k}": f"l{i}.mlp.{k}", f"layers.{i}.ff.{k}_bias": f"l{i}.mlp.{k}.b"})
+            if mlp["kind"] == "routed":
+                layer.experts = routed_experts(i, mlp, "silu", tensors)
+            else:
+                layer.ff, layer.ff_act, layer.ff_bias = mlp["ff"], "silu", True
+                for k in ("gate", "up", "down"):
+                    tensors.update({f"layers.{i}.ff.{k}": f"l{i}.mlp.{k}", f"layers.{i}.ff.{k}_bias": f"l{i}.mlp.{k}.b"})
         layers.append(layer)
     return StackSpec("Pabalix", cfg["vocab"], cfg["width"], layers, cfg["norm"]["eps"], plain_norm=True, post_norm=True, untied=True, tensors=tensors)

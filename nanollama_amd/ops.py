@@ -13,9 +13,7 @@ from __future__ import annotations
 import ctypes as C
 
 from . import _lib
-from .stack import ACTIVATIONS, DTYPES
-
-SCORES = {"softmax": 0, "sigmoid": 1}
+from .stack import ACTIVATIONS, DTYPES, SCORES
 
 
 def _type(a) -> str:

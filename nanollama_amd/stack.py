@@ -74,6 +74,20 @@ class LatentAttention:
 
 
 ACTIVATIONS = {"gelu_tanh": 0, "silu": 1}
+SCORES = {"softmax": 0, "sigmoid": 1}
+
+
+@dataclass
+class Experts:
+    """A feed-forward of experts, see nl_stack_experts_desc and nl_route_desc."""
+    experts: int
+    per_token: int
+    ff: int                     # width of an expert
+    act: str = "gelu_tanh"
+    score: str = "softmax"
+    renorm: bool = True
+    bias: bool = False
+    scale: float = 1.0
 
 
 @dataclass
@@ -84,6 +98,7 @@ class StackLayer:
     ff: int = 0
     ff_act: str = "gelu_tanh"
     ff_bias: bool = False
+    experts: Optional[Experts] = None                # instead of ff
 
     def mixers(self):
         return [m for m in (self.attn, self.lin, self.latent) if m]
@@ -121,7 +136,7 @@ class StackConfig:
         self.num_layers, self.embed_dim, self.vocab_size = len(spec.layers), spec.dim, spec.vocab
         self.num_heads = max(m.heads for l in spec.layers for m in l.mixers())
         self.num_kv_heads = max((l.attn.kv_heads for l in spec.layers if l.attn), default=0)
-        self.interm_size = max(l.ff for l in spec.layers)
+        self.interm_size = max(l.experts.per_token * l.experts.ff if l.experts else l.ff for l in spec.layers)
         self.rms_norm_eps = spec.eps
         self.qk_norm = any(l.attn and l.attn.qk_norm for l in spec.layers)
         self.rope_conjugate = False
@@ -193,12 +208,17 @@ def load_stack_model(spec: StackSpec, get: Callable[[str], Tuple[str, np.ndarray
         raise _lib.NlError(rc, (L.nl_last_error(None) or b"").decode())
     params = 0
     try:
+        for i, layer in enumerate(spec.layers):
+            if layer.experts:
+                x = layer.experts
+                d = _lib.NlStackExpertsDesc(x.experts, x.per_token, x.ff, ACTIVATIONS[x.act], SCORES[x.score], int(x.renorm), int(x.bias), x.scale)
+                _lib.check(h, L.nl_stack_experts(h, i, d), L)
         for name, source in spec.tensors.items():
             tag, x = get(source)
             if tag not in ("F32", "BF16"):
                 raise ValueError(f"tensor {source}: type {tag} (float32 and bfloat16 are taken)")
             x = np.ascontiguousarray(x)
-            rows, cols = (1, x.shape[0]) if x.ndim == 1 else x.shape
+            rows, cols = (1, x.shape[0]) if x.ndim == 1 else (x.size // x.shape[-1], x.shape[-1])      # (experts' matrices: expert behind expert)
             params += x.size
             _lib.check(h, L.nl_upload_tensor(h, name.encode(), 0 if tag == "F32" else 30, x.ctypes.data, x.nbytes, rows, cols), L)
         _lib.check(h, L.nl_finalize(h), L)

@@ -14,6 +14,19 @@ import numpy as np
 from .safetensors import save, to_bf16
 
 
+def routed(experts: int, per_token: int, ff: int, **more) -> dict:
+    """A feed-forward of experts as a layer's "mlp"; more: score, renorm, scale, bias."""
+    return {"kind": "routed", "experts": experts, "per_token": per_token, "ff": ff, **more}
+
+
+def _routed_shapes(p: str, mlp: dict, width: int) -> Dict[str, Tuple[int, ...]]:
+    E, f = mlp["experts"], mlp["ff"]
+    out: Dict[str, Tuple[int, ...]] = {p + "router": (E, width), p + "experts.gate": (E, f, width), p + "experts.up": (E, f, width), p + "experts.down": (E, width, f)}
+    if mlp.get("bias"):
+        out[p + "router.b"] = (E,)
+    return out
+
+
 def ganidra_layer(kind: str, width_mlp: int = 0, **mixer) -> dict:
     return {"type": kind, "mixer": mixer, "mlp": {"kind": "dense", "ff": width_mlp} if width_mlp else None}
 
@@ -48,13 +61,14 @@ def ganidra_shapes(cfg: dict, rank: int = 16) -> Dict[str, Tuple[int, ...]]:
             lin(p + "mix.right.", L["mixer"]["right"])
         if L["mlp"]:
             f = L["mlp"]["ff"]
-            out.update({p + "norm2": (D,), p + "mlp.gate": (f, D), p + "mlp.up": (f, D), p + "mlp.down": (D, f)})
+            out[p + "norm2"] = (D,)
+            out.update(_routed_shapes(p + "mlp.", L["mlp"], D) if L["mlp"]["kind"] == "routed" else {p + "mlp.gate": (f, D), p + "mlp.up": (f, D), p + "mlp.down": (D, f)})
     out["final.norm"] = (D,)
     return out
 
 
 def _fast_matrix(rng, shape, size: float) -> np.ndarray:
-    n = shape[0] * shape[1]
+    n = int(np.prod(shape))
     bits = rng.integers(0, 1 << 63, size=(n + 3) // 4, dtype=np.int64).view(np.uint16)[:n].reshape(shape)
     return (bits & np.uint16(0x807F)) | (np.uint16(127 + int(np.floor(np.log2(size)))) << np.uint16(7))
 
@@ -70,11 +84,13 @@ def ganidra_weights(cfg: dict, seed: int, rank: int = 16, gain: float = 1.0, fas
             x = 1.0 + 0.2 * rng.standard_normal(shape)
         elif name.endswith("a2.b"):
             x = rng.uniform(-3.0, 5.0, shape)
-        elif len(shape) == 2 and fast and not name.endswith(("a1", "a2")):
-            out[name] = _fast_matrix(rng, shape, gain / np.sqrt(shape[1] if name != "embed" else 1.0))
+        elif name.endswith("router.b"):
+            x = 0.3 * rng.standard_normal(shape)
+        elif len(shape) >= 2 and fast and not name.endswith(("a1", "a2")):
+            out[name] = _fast_matrix(rng, shape, gain / np.sqrt(shape[-1] if name != "embed" else 1.0))
             continue
         else:
-            x = rng.standard_normal(shape) * (1.0 if name == "embed" else gain / np.sqrt(shape[1]))
+            x = rng.standard_normal(shape) * (1.0 if name == "embed" else gain / np.sqrt(shape[-1]))
         out[name] = to_bf16(x.astype(np.float32))
     return out
 
@@ -110,7 +126,8 @@ def pabalix_shapes(cfg: dict) -> Dict[str, Tuple[int, ...]]:
             out.update({p + "sink": (H,), p + "g": (H, D)})
         if L["mlp"]:
             f, p = L["mlp"]["ff"], f"l{i}.mlp."
-            out.update({f"l{i}.norm2": (D,), f"l{i}.norm2b": (D,), p + "gate": (f, D), p + "gate.b": (f,), p + "up": (f, D), p + "up.b": (f,), p + "down": (D, f), p + "down.b": (D,)})
+            out.update({f"l{i}.norm2": (D,), f"l{i}.norm2b": (D,)})
+            out.update(_routed_shapes(p, L["mlp"], D) if L["mlp"]["kind"] == "routed" else {p + "gate": (f, D), p + "gate.b": (f,), p + "up": (f, D), p + "up.b": (f,), p + "down": (D, f), p + "down.b": (D,)})
     return out
 
 
@@ -119,11 +136,11 @@ def pabalix_weights(cfg: dict, seed: int, gain: float = 1.0, fast: bool = False)
     out = {}
     for name, shape in pabalix_shapes(cfg).items():
         rng = np.random.Generator(np.random.PCG64([seed, zlib.crc32(name.encode())]))
-        if len(shape) == 2 and fast:
-            out[name] = _fast_matrix(rng, shape, 1.0 if name == "embed" else gain / np.sqrt(max(1, shape[1])))
+        if len(shape) >= 2 and fast:
+            out[name] = _fast_matrix(rng, shape, 1.0 if name == "embed" else gain / np.sqrt(max(1, shape[-1])))
             continue
-        if len(shape) == 2:
-            x = rng.standard_normal(shape) * (1.0 if name == "embed" else gain / np.sqrt(max(1, shape[1])))
+        if len(shape) >= 2:
+            x = rng.standard_normal(shape) * (1.0 if name == "embed" else gain / np.sqrt(max(1, shape[-1])))
         elif "norm" in name:
             x = 1.0 + 0.2 * rng.standard_normal(shape)
         elif name.endswith("sink"):

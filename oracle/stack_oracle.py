@@ -101,6 +101,25 @@ def gated_mlp(h, w, p):
     return (gelu_tanh(h @ w[p + "gate"].T) * (h @ w[p + "up"].T)) @ w[p + "down"].T
 
 
+def routed_mlp(h, m, w, p, act):
+    """Experts: every token's per_token best of router h, their gated products weighted by the scores (over the sum of the chosen ones with renorm)."""
+    l = h @ w[p + "router"].T
+    if m.get("score", "softmax") == "softmax":
+        s = np.exp(l - l.max(axis=-1, keepdims=True))
+        s /= s.sum(axis=-1, keepdims=True)
+        key = l
+    else:
+        s = sigmoid(l)
+        key = s + w[p + "router.b"] if m.get("bias") else s
+    out = np.zeros_like(h)
+    for t in range(h.shape[0]):
+        ids = np.argsort(-key[t], kind="stable")[:m["per_token"]]
+        g = s[t, ids] / (s[t, ids].sum() if m.get("renorm", True) else 1.0) * m.get("scale", 1.0)
+        for e, a in zip(ids, g):
+            out[t] += a * (w[p + "experts.down"][e] @ (act(w[p + "experts.gate"][e] @ h[t]) * (w[p + "experts.up"][e] @ h[t])))
+    return out
+
+
 def layer_runs(cfg):
     """[(layer, add the embedding output first?)] in execution order."""
     n, loop = len(cfg["layers"]), cfg.get("loop")
@@ -203,7 +222,9 @@ def latent_forward(cfg, w, tokens, want_layers=False):
         o = latent_attention(h, m, w, p + "mix.", eps, L["type"], held[i if m.get("kv_from") is None else m["kv_from"]])
         x = x + norm_plain(o, w[p + "norm1b"], eps)
         if L["mlp"] is not None:
-            x = x + norm_plain(biased_silu_mlp(norm_plain(x, w[p + "norm2"], eps), w, p + "mlp."), w[p + "norm2b"], eps)
+            h = norm_plain(x, w[p + "norm2"], eps)
+            o = routed_mlp(h, L["mlp"], w, p + "mlp.", silu) if L["mlp"]["kind"] == "routed" else biased_silu_mlp(h, w, p + "mlp.")
+            x = x + norm_plain(o, w[p + "norm2b"], eps)
         seen.append(x)
     logits = norm_plain(x, w["final.norm"], eps) @ w["head"].T
     return (logits, np.stack(seen)) if want_layers else logits
@@ -223,7 +244,8 @@ def forward(cfg, w, tokens, want_layers=False):
         L, p = cfg["layers"][i], f"l{i}."
         x = x + MIXERS[L["type"]](norm_one_plus(x, w[p + "norm1"], eps), L["mixer"], w, p + "mix.", eps)
         if L["mlp"] is not None:
-            x = x + gated_mlp(norm_one_plus(x, w[p + "norm2"], eps), w, p + "mlp.")
+            h = norm_one_plus(x, w[p + "norm2"], eps)
+            x = x + (routed_mlp(h, L["mlp"], w, p + "mlp.", gelu_tanh) if L["mlp"]["kind"] == "routed" else gated_mlp(h, w, p + "mlp."))
         seen.append(x)
     logits = norm_one_plus(x, w["final.norm"], eps) @ w["embed"].T
     return (logits, np.stack(seen)) if want_layers else logits
