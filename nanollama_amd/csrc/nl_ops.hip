@@ -6,6 +6,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <algorithm>
+#include <atomic>
 #include <tuple>
 
 using namespace nl;
@@ -21,11 +22,19 @@ hipError_t start(void (*kernel)(F...), dim3 grid, dim3 block, size_t lds, hipStr
     return hipLaunchKernel(reinterpret_cast<const void *>(kernel), grid, block, at, lds, st);
 }
 
-// the same with more dynamic LDS than a kernel has by itself (asked for once a device and kernel; the flag is a hint, a second time does no harm)
-template <typename... F, typename... A>
-hipError_t start_lds(void (*kernel)(F...), dim3 grid, dim3 block, size_t lds, hipStream_t st, A... args) {
-    const hipError_t rc = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    return rc != hipSuccess ? rc : start(kernel, grid, block, lds, st, args...);
+// the same with more dynamic LDS than a kernel has by itself, which is asked for once a device
+template <auto *KERNEL, typename... A>
+hipError_t start_lds(dim3 grid, dim3 block, size_t lds, hipStream_t st, A... args) {
+    static std::atomic<unsigned long long> asked{0};
+    int device = 0;
+    hipError_t rc = hipGetDevice(&device);
+    if (rc != hipSuccess) return rc;
+    const unsigned long long bit = device < 64 ? 1ull << device : 0;
+    if (!(asked.load(std::memory_order_relaxed) & bit)) {
+        if ((rc = hipFuncSetAttribute(reinterpret_cast<const void *>(KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds)) != hipSuccess) return rc;
+        asked.fetch_or(bit, std::memory_order_relaxed);
+    }
+    return start(KERNEL, grid, block, lds, st, args...);
 }
 
 inline bool on16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -68,7 +77,7 @@ template <typename T, bool FIRST, typename S> static hipError_t grouped(const Ex
     const int slots = P.n * P.k, hit = std::min(P.experts, slots), rows = FIRST ? P.ff : P.dim, br = S::RT * (FIRST ? 8 : 16);
     const long long most = ((hit + (slots - hit) / S::BT) * (long long)((rows + br - 1) / br) + 7) / 8 * 8;
     if (most > INT_MAX / S::THREADS) return hipErrorInvalidConfiguration;
-    return start_lds(experts_many_kernel<T, FIRST, S>, dim3((unsigned)most), dim3(S::THREADS), S::LDS, st, P);
+    return start_lds<experts_many_kernel<T, FIRST, S>>(dim3((unsigned)most), dim3(S::THREADS), S::LDS, st, P);
 }
 // What tiles of S are expected to take, in us: rounds of workgroups over the CUs x (stages + what a workgroup has in front of and behind them).
 template <bool FIRST, typename S> static double grouped_us(const ExpertsParams &P, double stage) {
@@ -173,8 +182,12 @@ struct OnDevice {
 
 // what every operator checks behind its own arguments, then the launches
 template <typename F> int on_device(const char *name, int device, void *stream, F launches) {
-    int ndev = 0;
-    if (hipGetDeviceCount(&ndev) != hipSuccess || ndev == 0) return fail(NL_ERR_HIP, "%s: no HIP device", name);
+    static std::atomic<int> seen{0};                     // devices, once there are any
+    int ndev = seen.load(std::memory_order_relaxed);
+    if (ndev == 0) {
+        if (hipGetDeviceCount(&ndev) != hipSuccess || ndev == 0) return fail(NL_ERR_HIP, "%s: no HIP device", name);
+        seen.store(ndev, std::memory_order_relaxed);
+    }
     if (device < 0 || device >= ndev) return fail(NL_ERR_INVALID, "%s: device %d of %d", name, device, ndev);
     OnDevice on(device);
     if (on.rc != hipSuccess) return fail(NL_ERR_HIP, "%s: %s", name, hipGetErrorString(on.rc));

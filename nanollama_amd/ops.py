@@ -10,35 +10,53 @@ imported): outputs are passed in, rows may be further apart than they are long, 
 """
 from __future__ import annotations
 
-import ctypes as C
+from functools import lru_cache
 
 from . import _lib
 from .stack import ACTIVATIONS, DTYPES, SCORES
 
 
+_names: dict = {}               # an array library's type -> its name
+
+
 def _type(a) -> str:
-    return str(a.dtype).rpartition(".")[2]
+    t = _names.get(a.dtype)
+    if t is None:
+        t = _names[a.dtype] = str(a.dtype).rpartition(".")[2]
+    return t
 
 
-def _array(name: str, a, dtype: str, shape, device=None, strided=False):
+def _array(name: str, a, dtype: str, shape: tuple, device=None, strided=False):
     """Pointer and row distance of an array that has to have this type and shape."""
-    if _type(a) != dtype:
+    if _names.get(a.dtype) != dtype and _type(a) != dtype:
         raise ValueError(f"{name}: type {_type(a)}, expected {dtype}")
-    if tuple(a.shape) != tuple(shape):
+    if a.shape != shape:
         raise ValueError(f"{name}: shape {list(a.shape)}, expected {list(shape)}")
     if device is not None and a.device.index != device:
         raise ValueError(f"{name}: on device {a.device.index}, the others on {device}")
-    stride, dense = a.stride(), 1
-    for i in range(len(shape) - 1, -1, -1):
-        if shape[i] > 1 and stride[i] != dense and not (strided and i == 0 and len(shape) == 2 and stride[i] >= dense):
+    stride = a.stride()
+    if stride[-1] == 1 and len(shape) <= 2:              # (nearly always)
+        if len(shape) == 1 or stride[0] == shape[1]:
+            return a.data_ptr(), shape[-1]
+        if strided and shape[0] > 1 and stride[0] > shape[1]:
+            return a.data_ptr(), stride[0]
+    dense = 1
+    for n, s in zip(reversed(shape), reversed(stride)):
+        if n > 1 and s != dense:
             raise ValueError(f"{name}: elements are not dense" + (" within a row" if strided else ""))
-        dense *= shape[i]
-    return a.data_ptr(), stride[0] if strided and shape[0] > 1 else shape[-1]
+        dense *= n
+    return a.data_ptr(), shape[-1]
 
 
 def _check(rc: int) -> None:
     if rc != 0:
         raise _lib.NlError(rc, (_lib.stack_lib().nl_last_error(None) or b"").decode())
+
+
+@lru_cache(maxsize=256)
+def _desc(kind, *fields):
+    """A description; the library only reads it."""
+    return kind(*fields)
 
 
 def _one_of(name: str, value: str, table) -> int:
@@ -54,13 +72,13 @@ def route(logits, ids, weights, score: str = "softmax", bias=None, renorm: bool 
     ip, _ = _array("ids", ids, "int32", (n, k), dev)
     wp, _ = _array("weights", weights, "float32", (n, k), dev)
     bp = None if bias is None else _array("bias", bias, "float32", (count,), dev)[0]
-    d = _lib.NlRouteDesc(count, k, _one_of("score", score, SCORES), int(renorm), scale)
+    d = _desc(_lib.NlRouteDesc, count, k, _one_of("score", score, SCORES), int(renorm), scale)
     _check(_lib.stack_lib().nl_op_route(dev, stream, d, n, lp, ld, bp, ip, wp))
 
 
 def experts_workspace(n: int, per_token: int, count: int, dim: int, ff: int, dtype: str = "bfloat16") -> int:
     """Bytes that experts() needs beside its arrays for up to n tokens."""
-    d = _lib.NlExpertsDesc(count, per_token, dim, ff, 0, _one_of("dtype", dtype, DTYPES))
+    d = _desc(_lib.NlExpertsDesc, count, per_token, dim, ff, 0, _one_of("dtype", dtype, DTYPES))
     size = _lib.stack_lib().nl_op_experts_workspace(d, n)
     if size == 0:
         _check(-1)
@@ -80,7 +98,7 @@ def experts(x, ids, weights, gate, up, down, out, workspace, act: str = "silu", 
     yp, ldy = _array("out", out, t, (n, dim), dev, strided=True)
     size = workspace.numel()
     sp, _ = _array("workspace", workspace, "uint8", (size,), dev)
-    d = _lib.NlExpertsDesc(count, k, dim, ff, _one_of("act", act, ACTIVATIONS), _one_of("type of x", t, DTYPES))
+    d = _desc(_lib.NlExpertsDesc, count, k, dim, ff, _one_of("act", act, ACTIVATIONS), _one_of("type of x", t, DTYPES))
     _check(_lib.stack_lib().nl_op_experts(dev, stream, d, n, xp, ldx, ip, wp, gp, up_, dp, yp, ldy, sp, size))
 
 
@@ -98,5 +116,5 @@ def residual_norm(x, d, x_out, h=None, pre=None, post=None, gate=None, scale: fl
     gp, ldg = None, 0
     if gate is not None:
         gp, ldg = (vec("gate", gate), 0) if len(gate.shape) == 1 else _array("gate", gate, "float32", (n, dim), dev, strided=True)
-    desc = _lib.NlResidualNormDesc(dim, _one_of("type of d", t, DTYPES), eps, scale)
+    desc = _desc(_lib.NlResidualNormDesc, dim, _one_of("type of d", t, DTYPES), eps, scale)
     _check(_lib.stack_lib().nl_op_residual_norm(dev, stream, desc, n, xp, ldx, dp, ldd, vec("post", post), gp, ldg, vec("pre", pre), op, ldo, hp, ldh))
