@@ -161,11 +161,14 @@ __global__ void __launch_bounds__(1024) plan_kernel(const int *ids, int nslots, 
     const int e = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int per = ((nslots + 15) / 16 + 63) & ~63, lo = min(w * per, nslots), hi = min(lo + per, nslots);      // this wavefront's slots
     int nl = 0, nm = 0;
-    for (int s = lo; s < hi; s += 64) {
-        const int id = s + lane < hi ? ids[s + lane] : -1;
-        nl += __popcll(__ballot(id >= 0 && id < e));
-        nm += __popcll(__ballot(id == e));
+#pragma unroll 8
+    for (int s = lo + lane; s < hi; s += 64) {           // (a lane counts for itself: its loads do not wait for one another)
+        const int id = ids[s];
+        nl += id >= 0 && id < e;
+        nm += id == e;
     }
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) { nl += __shfl_xor(nl, s); nm += __shfl_xor(nm, s); }
     if (lane == 0) { less[w] = nl; mine[w] = nm; }
     __syncthreads();
     int at = 0, before = 0, all = 0;
@@ -179,11 +182,17 @@ __global__ void __launch_bounds__(1024) plan_kernel(const int *ids, int nslots, 
         if (e == experts - 1) offs[experts] = at + all;
     }
     at += before;
-    for (int s = lo; s < hi; s += 64) {
-        const int id = s + lane < hi ? ids[s + lane] : -1;
-        const unsigned long long m = __ballot(id == e);
-        if (id == e) order[at + __popcll(m & ((1ull << lane) - 1))] = s + lane;
-        at += __popcll(m);
+    constexpr int U = 8;
+    for (int s = lo; s < hi; s += 64 * U) {
+        int id[U];
+#pragma unroll
+        for (int i = 0; i < U; i++) id[i] = s + i * 64 + lane < hi ? ids[s + i * 64 + lane] : -1;
+#pragma unroll
+        for (int i = 0; i < U; i++) {
+            const unsigned long long m = __ballot(id[i] == e);
+            if (id[i] == e) order[at + __popcll(m & ((1ull << lane) - 1))] = s + i * 64 + lane;
+            at += __popcll(m);
+        }
     }
 }
 
@@ -350,8 +359,8 @@ __global__ void __launch_bounds__(256) experts_token_second_kernel(ExpertsParams
 // 1 KiB piece is 8 rows x 128 bytes, whole lines of the rows as they lie; in LDS the 16-byte run q of row r is at q ^ (r % 8), so that the 16 rows of a
 // fragment are read from all banks.  FIRST: row tiles alternate between gate and up.
 // Workgroups b, b + 8, ... run on one XCD and take a contiguous range of (expert, row block, token tile): both operands of neighbours are in its L2.
-template <typename T, int RTW_, int NTW_, int WR_, int WT_> struct Grouped {
-    static constexpr int RTW = RTW_, NTW = NTW_, WR = WR_, WT = WT_, RT = WR * RTW, NT = WT * NTW, STAGE = (RT + NT) * 2048, LDS = 2 * STAGE, NW = WR * WT, THREADS = 64 * NW,
+template <typename T, int RTW_, int NTW_, int WR_, int WT_, int NST_ = 2> struct Grouped {
+    static constexpr int NST = NST_, RTW = RTW_, NTW = NTW_, WR = WR_, WT = WT_, RT = WR * RTW, NT = WT * NTW, STAGE = (RT + NT) * 2048, LDS = NST * STAGE, NW = WR * WT, THREADS = 64 * NW,
                          PW = STAGE / 1024 / NW, BT = NT * 16, KB = 128 / (int)sizeof(T), KK = KB / 32, PER_CU = 163840 / LDS;
     static_assert(PW * NW * 1024 == STAGE, "pieces");
 };
@@ -370,7 +379,7 @@ template <> __device__ __forceinline__ Frag<float> swizzled_frag<float>(const ch
 }
 template <typename T, bool FIRST, typename S>
 __global__ void __launch_bounds__(S::THREADS, S::NW * S::PER_CU / 4) experts_many_kernel(ExpertsParams P) {
-    constexpr int RT = S::RT, STAGE = S::STAGE, NW = S::NW, PW = S::PW, BT = S::BT, KB = S::KB, KK = S::KK, RTW = S::RTW, NTW = S::NTW;
+    constexpr int RT = S::RT, NST = S::NST, STAGE = S::STAGE, NW = S::NW, PW = S::PW, BT = S::BT, KB = S::KB, KK = S::KK, RTW = S::RTW, NTW = S::NTW;
     constexpr int BR = (FIRST ? RT / 2 : RT) * 16;        // output rows of the workgroup
     extern __shared__ __align__(16) char lds[];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15, wr = w % S::WR, wt = w / S::WR;
@@ -391,11 +400,11 @@ __global__ void __launch_bounds__(S::THREADS, S::NW * S::PER_CU / 4) experts_man
     const int turn = rb * nks / nrb;                     // (row blocks start at different columns: their rows would else ask the same memory channels)
     const char *src[PW];
     const int k0 = ((lane & 7) ^ (lane >> 3)) * (16 / (int)sizeof(T));
-    int there = 0;                                       // pieces with a token or a row of the matrix: the first ones
+    int there = NST == 2 ? 0 : PW;                       // pieces with a token or a row of the matrix: the first ones (all, where waits count them)
 #pragma unroll
     for (int i = 0; i < PW; i++) {
         const int u = i * NW + w;
-        if ((u >> 1) < RT || ((u >> 1) - RT) * 16 + (u & 1) * 8 < count) there = i + 1;
+        if (NST == 2 && ((u >> 1) < RT || ((u >> 1) - RT) * 16 + (u & 1) * 8 < count)) there = i + 1;
         src[i] = reinterpret_cast<const char *>(row_of(u >> 1, (u & 1) * 8 + (lane >> 3)) + k0);
     }
     auto issue = [&](int ks, int st) {
@@ -423,22 +432,28 @@ __global__ void __launch_bounds__(S::THREADS, S::NW * S::PER_CU / 4) experts_man
     };
     auto multiply = [&](const Frag<T> *a, const Frag<T> *b) {
 #pragma unroll
-        for (int r = 0; r < RTW; r++)
+        for (int t = 0; t < NTW; t++) {
+            if (sizeof(T) == 4 && (wt * NTW + t) * 16 >= count) break;       // (32 bits: the matrix rate bounds it; for 16 the branches cost more)
 #pragma unroll
-            for (int t = 0; t < NTW; t++) acc[r][t] = mma(a[r], b[t], acc[r][t]);
+            for (int r = 0; r < RTW; r++) acc[r][t] = mma(a[r], b[t], acc[r][t]);
+        }
     };
     // (builtins, not lds_barrier(): the compiler has to know that nothing is on its way from LDS, or it waits for the next fragments before it
     // multiplies the present ones)
     auto arrived = [&]() { __builtin_amdgcn_s_waitcnt(0xc07f); };
+    int st = 0;
     auto next_stage = [&](int s) {                       // to stage s < nks; the one before it is read and filled again
-        vm_wait<0>();
+        if (NST > 2 && nks - 1 - s >= NST - 2) vm_wait<PW *(NST - 2)>();
+        else vm_wait<0>();
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if (s + 1 < nks) issue(s + 1, (s + 1) & 1);
+        if (s - 1 + NST < nks) issue(s - 1 + NST, st);
+        st = st + 1 == NST ? 0 : st + 1;
     };
-    issue(0, 0);
-    if (nks > 1) issue(1, 1);
-    if (nks > 1 && there == PW) vm_wait<PW>();
+#pragma unroll
+    for (int s = 0; s < NST; s++)
+        if (s < nks) issue(s, s);
+    if (nks >= NST && there == PW) vm_wait<PW *(NST - 1)>();
     else vm_wait<0>();
     lds_barrier();
     if (!busy) {
@@ -451,7 +466,7 @@ __global__ void __launch_bounds__(S::THREADS, S::NW * S::PER_CU / 4) experts_man
     for (int s = 0; s + 1 < nks; s++) {
         arrived();
         if constexpr (KK == 2) {
-            read(s & 1, 1, fa[1], fb[1]);
+            read(st, 1, fa[1], fb[1]);
             __builtin_amdgcn_sched_barrier(0);
             multiply(fa[0], fb[0]);
             __builtin_amdgcn_sched_barrier(0);
@@ -459,16 +474,16 @@ __global__ void __launch_bounds__(S::THREADS, S::NW * S::PER_CU / 4) experts_man
         }
         next_stage(s + 1);
         if constexpr (KK == 2) {
-            read(~s & 1, 0, fa[0], fb[0]);
+            read(st, 0, fa[0], fb[0]);
             __builtin_amdgcn_sched_barrier(0);
             multiply(fa[1], fb[1]);
         } else {
             multiply(fa[0], fb[0]);
-            read(~s & 1, 0, fa[0], fb[0]);
+            read(st, 0, fa[0], fb[0]);
         }
         __builtin_amdgcn_sched_barrier(0);
     }
-    if constexpr (KK == 2) read((nks - 1) & 1, 1, fa[1], fb[1]);
+    if constexpr (KK == 2) read(st, 1, fa[1], fb[1]);
     multiply(fa[0], fb[0]);
     if constexpr (KK == 2) multiply(fa[1], fb[1]);
 #pragma unroll

@@ -79,31 +79,46 @@ template <typename T, bool FIRST, typename S> static hipError_t grouped(const Ex
     if (most > INT_MAX / S::THREADS) return hipErrorInvalidConfiguration;
     return start_lds<experts_many_kernel<T, FIRST, S>>(dim3((unsigned)most), dim3(S::THREADS), S::LDS, st, P);
 }
-// What tiles of S are expected to take, in us: rounds of workgroups over the CUs x (stages + what a workgroup has in front of and behind them).
-template <bool FIRST, typename S> static double grouped_us(const ExpertsParams &P, double stage) {
-    const double slots = (double)P.n * P.k, hit = std::min<double>(P.experts, slots), tiles = std::max(hit, slots / S::BT + hit / 2);
+// What tiles of S are expected to take (bfloat16), in us.  A CU runs its workgroups in rounds of S::PER_CU; a stage of a round takes what bounds it: bringing
+// it to LDS (50 KB/us and CU), multiplying it (`tflops` a CU), reading the matrices' part (6.2 TB/s), or the way from
+// memory as far as the ring does not hide it; `around`: what is in front of the stages and behind them.
+template <bool FIRST, typename S> static double grouped_us(const ExpertsParams &P, double tflops, double around) {
     const int rows = FIRST ? P.ff : P.dim, K = FIRST ? P.dim : P.ff, br = S::RT * (FIRST ? 8 : 16);
-    return std::ceil(tiles * ((rows + br - 1) / br) / (256 * S::PER_CU)) * (stage * ((K + S::KB - 1) / S::KB) + 5);
+    const double slots = (double)P.n * P.k, hit = std::min<double>(P.experts, slots), tiles = std::max(hit, slots / S::BT + hit / 2), per_tile = std::min<double>(S::BT, slots / tiles);
+    const double all = tiles * ((rows + br - 1) / br), round = 256 * S::PER_CU, stages = (K + S::KB - 1) / S::KB;
+    const double bring = (S::RT * 16 + per_tile) * 128 / 50e3, multiply = 2 * S::RT * 16 * std::max(32., std::min<double>(S::BT, per_tile + 16)) * S::KB / (tflops * 1e6);
+    const double read = hit / tiles * S::RT * 16 * 128 / 6.2e6, way = S::NST > 2 ? 0.29 : 0.92;
+    auto took = [&](double workgroups) {
+        const double a_cu = std::ceil(workgroups / 256);
+        return stages * std::max(std::max(a_cu * bring, a_cu * multiply), std::max(workgroups * read, way)) + around;
+    };
+    const double full = std::floor(all / round), left = all - full * round;
+    return full * took(round) + (left > 0 ? took(left) : 0);
 }
-// Which tiles.  bfloat16, rows x tokens 128 x 64 (three workgroups a CU), 128 x 128 (two) or 256 x 256 (one), whichever is expected to be done first;
-// a stage takes 1.05, 1.05 and 1.8 us there.  us measured of a product with gate and up / with down:
-//   64 experts of 1536 x 768, 8 a token, 2047 tokens   150 / 100   125 / 86   139 / 97        512 tokens   77 / 45   75 / 46   87 / 52
-//   8 of 4096 x 11008, 2 a token, 993 tokens           -           549 / 444  567 / 314       256 tokens   297 / 183  312 / 201  329 / 260
-//   8 of 768 x 2048, 2 a token, 1000 tokens            30 / 30     31 / 33    29 / 55
-// 64 x 64 where 128 x 64 has no workgroup for every CU: down of the last at 333 tokens 18.5 instead of 21.4; but 28 instead of 23 at 16 tokens of the first,
-// which has 672.  32 bits: always 64 x 64, bound by the matrix rate (77 tokens to 4 of 16 of 760 x 500: 23 / 16, with 128 x 64 35 / 24, 128 x 128 55 / 38;
-// 1024 tokens of the first 521 / 265, 527 / 267, 596 / 319).
+// Which tiles.  bfloat16: rows x tokens 64 x 64 in three stages (three workgroups a CU), 128 x 64 in two (three), 128 x 128 (two) or 256 x 256 (one), whichever
+// is expected to be done first: 1 % behind the best of the four on the average over 54 measured products.  us of a product with gate and up / with down:
+//                                                                     64 x 64     128 x 64    128 x 128   256 x 256
+//   64 experts of 1536 x 768, 8 a token        32 tokens              49 / 27     49 / 25     61 / 32     74 / 40
+//                                              512                    82 / 47     78 / 47     76 / 47     87 / 53
+//                                              2047                   182 / 118   148 / 100   126 / 87    143 / 99
+//   64 of 1536 x 1024, 6 a token               64                     66 / 35     79 / 33     68 / 42     82 / 47
+//   8 of 768 x 2048, 2 a token                 333                    17 / 13     15 / 22     17 / 25     24 / 50
+//                                              1000                   33 / 21     30 / 30     30 / 33     29 / 56
+//   8 of 4096 x 11008, 2 a token               16                     224 / 108   215 / 152   237 / 155   259 / 209
+//                                              993                    783 / 431   634 / 409   559 / 447   587 / 335
+// 32 bits: 64 x 64, bound by the matrix rate (77 tokens to 4 of 16 of 760 x 500: 23 / 16, with 128 x 64 35 / 24, 128 x 128 55 / 38; 1024 tokens of the first
+// experts 521 / 265, 527 / 267, 596 / 319).
 template <typename T, bool FIRST> static hipError_t grouped_product(const ExpertsParams &P, hipStream_t st) {
-    using Small = Grouped<T, 2, 2, 2, 2>;
+    using Small = Grouped<T, 2, 2, 2, 2, 3>;
     if constexpr (sizeof(T) == 2) {
         using Low = Grouped<T, 4, 2, 2, 2>;
         using Square = Grouped<T, 4, 4, 2, 2>;
         using Large = Grouped<T, 8, 4, 2, 4>;
-        const double low = grouped_us<FIRST, Low>(P, 1.05), square = grouped_us<FIRST, Square>(P, 1.05);
-        if (grouped_us<FIRST, Large>(P, 1.8) < std::min(low, square)) return grouped<T, FIRST, Large>(P, st);
-        if (square < low) return grouped<T, FIRST, Square>(P, st);
-        const int slots = P.n * P.k, rows = FIRST ? P.ff : P.dim, br = Low::RT * (FIRST ? 8 : 16);
-        if (std::min(P.experts, slots) + slots / Low::BT / 2 > 256 / ((rows + br - 1) / br)) return grouped<T, FIRST, Low>(P, st);
+        const double small = grouped_us<FIRST, Small>(P, 5.4, 2.9), low = grouped_us<FIRST, Low>(P, 5.4, 2.9), square = grouped_us<FIRST, Square>(P, 5.4, 2.9), large = grouped_us<FIRST, Large>(P, 3.3, 8.1);
+        const double least = std::min(std::min(small, low), std::min(square, large));
+        if (large == least) return grouped<T, FIRST, Large>(P, st);
+        if (square == least) return grouped<T, FIRST, Square>(P, st);
+        if (low == least) return grouped<T, FIRST, Low>(P, st);
     }
     return grouped<T, FIRST, Small>(P, st);
 }

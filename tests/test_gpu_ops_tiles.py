@@ -1,0 +1,78 @@
+"""The experts' products in every size of tile, and slot by slot, at the sizes where one ends (nanollama_amd.ops.experts)."""
+import numpy as np
+import pytest
+
+from hip_arrays import Stream, sync
+from test_gpu_ops import Experts
+
+pytestmark = pytest.mark.gpu
+
+
+def skewed(n, E, k, seed=0):
+    """Experts asked for very differently, and places without one."""
+    rng = np.random.default_rng(seed)
+    ids = np.minimum(rng.geometric(3.0 / E, (n, k)) - 1, E + 1).astype(np.int32)      # E and E + 1 are no experts
+    ids[rng.random((n, k)) < 0.05] = -1
+    return ids
+
+
+# what is expected to be done first: 64 x 64 twice; 128 x 128 and 128 x 64; 128 x 64 and 128 x 128; 256 x 256 and 128 x 128; 128 x 128 and 64 x 64
+@pytest.mark.parametrize("n, dim, ff, E, k", [(600, 264, 200, 64, 8), (1500, 520, 1032, 16, 4), (700, 776, 520, 64, 4), (1600, 1032, 2056, 4, 2), (1600, 520, 1544, 4, 2)])
+def test_every_tile(n, dim, ff, E, k):
+    Experts(n, dim, ff, E, k, "bfloat16", seed=n).run()
+    Experts(n, dim, ff, E, k, "bfloat16", seed=n, ids=skewed(n, E, k), x_apart=dim + 8, y_apart=dim + 3).run()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("cols", [8, 24, 56, 64, 72, 120, 128, 136, 192, 200, 256])
+def test_rows_that_end_within_a_stage(cols, dtype):
+    Experts(70, cols, 64, 3, 2, dtype, seed=cols).run()
+    Experts(70, 64, cols, 3, 2, dtype, seed=cols).run()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("n", [15, 16, 17, 31, 33, 47, 49, 63, 64, 65, 127, 128, 129, 255, 256, 257])
+def test_groups_that_end_within_a_tile(n, dtype):
+    Experts(n, 64, 72, 2, 1, dtype, seed=n, ids=np.zeros((n, 1), np.int32)).run()
+    Experts(n, 64, 72, 3, 2, dtype, seed=n, ids=np.tile(np.array([[2, 0]], np.int32), (n, 1))).run()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("n, E, k", [(1, 1, 1), (1, 2, 2), (1, 40, 32), (1, 64, 8), (2, 8, 2), (2, 7, 2), (4, 64, 8), (5, 64, 8), (16, 1024, 32), (17, 1024, 32)])
+@pytest.mark.parametrize("dim, ff", [(8, 8), (264, 136), (1032, 520)])
+def test_a_few_tokens(n, E, k, dim, ff, dtype):
+    if E * dim * ff > 1 << 25:
+        dim, ff = 40, 24
+    Experts(n, dim, ff, E, k, dtype, seed=n).run()
+    Experts(n, dim, ff, E, k, dtype, seed=n, ids=np.random.default_rng(n).integers(-1, E + 1, (n, k))).run()
+    m = Experts(n, dim, ff, E, k, dtype, ids=np.full((n, k), -1), y_apart=dim + 5)
+    m.run()
+    assert np.all(m.y.numpy() == 0)
+
+
+def test_a_few_tokens_in_a_graph():
+    s = Stream()
+    m = Experts(2, 96, 64, 16, 4, "bfloat16")
+    play = s.capture(lambda: m.queue(s.number))
+    for i in range(4):
+        m.ids = np.random.default_rng(i).integers(-1, 16, m.ids.shape).astype(np.int32)
+        m.di.write(m.ids)
+        sync()
+        play()
+        s.sync()
+        m.check()
+        m.queue()                                          # eager work between the replays
+        sync()
+        m.check()
+
+
+def test_the_same_bits_every_time_with_every_tile():
+    for n, dim, ff, E, k in ((1500, 520, 1032, 16, 4), (700, 776, 520, 64, 4), (300, 264, 200, 6, 2), (1, 264, 200, 6, 2)):
+        m = Experts(n, dim, ff, E, k, "bfloat16", seed=n)
+        m.queue()
+        sync()
+        first = m.y.bits()
+        for _ in range(3):
+            m.queue()
+            sync()
+            assert np.array_equal(first, m.y.bits())
