@@ -435,7 +435,9 @@ __global__ void __launch_bounds__(S::THREADS, S::NW * S::PER_CU / 4) experts_man
         for (int t = 0; t < NTW; t++) {
             if (sizeof(T) == 4 && (wt * NTW + t) * 16 >= count) break;       // (32 bits: the matrix rate bounds it; for 16 the branches cost more)
 #pragma unroll
-            for (int r = 0; r < RTW; r++) acc[r][t] = mma(a[r], b[t], acc[r][t]);
+            for (int r = 0; r < RTW; r++)                // (32 bits: a stage's 32 products by themselves, then into the sum: one chain over the row is off by twice as much)
+                if constexpr (sizeof(T) == 4) acc[r][t] += mma(a[r], b[t], f32x4{});
+                else acc[r][t] = mma(a[r], b[t], acc[r][t]);
         }
     };
     // (builtins, not lds_barrier(): the compiler has to know that nothing is on its way from LDS, or it waits for the next fragments before it
