@@ -201,15 +201,16 @@ __global__ void __launch_bounds__(1024) plan_kernel(const int *ids, int nslots, 
 struct Group { int e, before, a, b; };
 template <int BT>
 struct Groups {
-    int per, mine, upto;
+    int per, lo, hi, mine, upto;
     const int *offs;
     __device__ __forceinline__ Groups(const int *o, int experts) : offs(o) {
         const int lane = threadIdx.x & 63, e0 = lane * (per = (experts + 63) >> 6);
         mine = 0;
-        for (int i = 0, a = offs[min(e0, experts)]; i < per; i++) {
+        hi = lo = offs[min(e0, experts)];
+        for (int i = 0; i < per; i++) {
             const int b = offs[min(e0 + i + 1, experts)];
-            mine += (b - a + BT - 1) / BT;
-            a = b;
+            mine += (b - hi + BT - 1) / BT;
+            hi = b;
         }
         upto = mine;
 #pragma unroll
@@ -224,7 +225,11 @@ struct Groups {
         Group G;
         G.before = __builtin_amdgcn_readlane(upto - mine, at);
         G.e = at * per;
-        G.a = __builtin_amdgcn_readfirstlane(offs[G.e]);
+        G.a = __builtin_amdgcn_readlane(lo, at);
+        if (per == 1) {
+            G.b = __builtin_amdgcn_readlane(hi, at);
+            return G;
+        }
         for (;;) {
             G.b = __builtin_amdgcn_readfirstlane(offs[G.e + 1]);
             const int n = (G.b - G.a + BT - 1) / BT;
