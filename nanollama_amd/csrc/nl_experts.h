@@ -457,7 +457,11 @@ __global__ void __launch_bounds__(256) experts_token_second_kernel(ExpertsParams
     sum = wave_sum(sum);
     if (lane != 0) return;
     if (P.y) put(reinterpret_cast<T *>(P.y) + (long long)t * P.ldy + row, sum);
-    else P.part[(long long)t * P.dim + row] = sum;
+    else if (P.res_out) {
+        float x = P.res[(long long)t * P.ldres + row];
+        if (P.add) x += P.add[(long long)t * P.ldadd + row];
+        P.res_out[(long long)t * P.ldo + row] = fmaf(P.scale, sum, x);
+    } else P.part[(long long)t * P.dim + row] = sum;
 }
 
 // Prompts: WR x WT wavefronts of RTW row tiles x NTW token tiles each; 128 bytes of every row at a time go through two LDS stages by LDS-DMA.  A

@@ -28,8 +28,12 @@ struct ExpertsParams {
     int *offs, *order;                    // first place of every expert [experts + 1]; place -> slot (token * k + j)
     void *h;                              // [place][ff] activations
     float *part;                          // [slot][dim] weighted results
-    void *y;                              // launch_experts has these
-    long long ldy;
+    // launch_experts has these: where the sums of a few tokens go at once, if anywhere
+    void *y;
+    const float *res, *add;
+    float *res_out;
+    long long ldy, ldres, ldadd, ldo;
+    float scale;
 };
 // bytes of the workspace and where its parts start
 struct ExpertsLayout { size_t offs, order, h, part, bytes; };
@@ -55,7 +59,7 @@ struct CloseParams {
     float eps, scale;
 };
 hipError_t launch_close(const CloseParams &P, int dtype, hipStream_t st);
-// the experts' products of P's tokens and the close C of their sums (its part, ids, k, experts, n and dim are filled in)
+// the experts' products of P's tokens and the close C of their sums (its part, ids, k, experts, n and dim are filled in, base and d stay null)
 hipError_t launch_experts(ExpertsParams P, CloseParams C, int dtype, hipStream_t st);
 
 }  // namespace nl

@@ -159,10 +159,13 @@ template <typename T> static hipError_t close(const CloseParams &P, hipStream_t 
 hipError_t launch_close(const CloseParams &P, int dtype, hipStream_t st) { return dtype == NL_DTYPE_F32 ? close<float>(P, st) : close<bf16>(P, st); }
 hipError_t launch_experts(ExpertsParams P, CloseParams C, int dtype, hipStream_t st) {
     C.part = P.part; C.ids = P.ids; C.k = P.k; C.experts = P.experts; C.n = P.n; C.dim = P.dim;
-    if (!C.x_out && !C.base) { P.y = C.y; P.ldy = C.ldy; }
+    P.y = C.x_out ? nullptr : C.y;
+    P.ldy = C.ldy;
+    P.res_out = C.post || C.gate || C.h ? nullptr : C.x_out;       // (nothing that needs the whole row)
+    P.ldo = C.ldxo; P.res = C.x; P.ldres = C.ldx; P.add = C.add; P.ldadd = C.ldadd; P.scale = C.scale;
     bool summed = false;
     const hipError_t rc = dtype == NL_DTYPE_F32 ? experts<float>(P, summed, st) : experts<bf16>(P, summed, st);
-    if (rc != hipSuccess || (summed && P.y)) return rc;
+    if (rc != hipSuccess || (summed && (P.y || P.res_out))) return rc;
     if (summed) { C.ids = nullptr; C.k = 1; }
     return launch_close(C, dtype, st);
 }
