@@ -106,10 +106,10 @@ template <bool FIRST, typename S> static double grouped_us(const ExpertsParams &
 //                                              1000                   33 / 21     30 / 30     30 / 33     29 / 56
 //   8 of 4096 x 11008, 2 a token               16                     224 / 108   215 / 152   237 / 155   259 / 209
 //                                              993                    783 / 431   634 / 409   559 / 447   587 / 335
-// 32 bits: 64 x 64, bound by the matrix rate (77 tokens to 4 of 16 of 760 x 500: 23 / 16, with 128 x 64 35 / 24, 128 x 128 55 / 38; 1024 tokens of the first
-// experts 521 / 265, 527 / 267, 596 / 319).
+// 32 bits: 64 x 32 in three stages, bound by the matrix rate; 64 x 64 and 128 x 128 beside it: 77 tokens to 4 of 16 of 760 x 500 21 / 11, 22 / 15, 55 / 38; of the
+// first experts 256 tokens 166 / 87, 208 / 110, 385 / 198, 1024 tokens 507 / 260, 496 / 259, 596 / 319.
 template <typename T, bool FIRST> static hipError_t grouped_product(const ExpertsParams &P, hipStream_t st) {
-    using Small = Grouped<T, 2, 2, 2, 2, 3>;
+    using Small = Grouped<T, 2, sizeof(T) == 2 ? 2 : 1, 2, 2, 3>;
     if constexpr (sizeof(T) == 2) {
         using Low = Grouped<T, 4, 2, 2, 2>;
         using Square = Grouped<T, 4, 4, 2, 2>;
