@@ -52,7 +52,8 @@ typedef struct {
 } nl_experts_desc;
 /* x [n][ldx], ids and weights [n][per_token], gate and up [experts][ff][dim], down [experts][dim][ff], y [n][ldy].  An id outside
  * [0, experts) adds nothing, whatever its weight (a row without any: y = 0); an id twice in a row counts twice.  Rows of y behind n are
- * not touched.  bfloat16: the activation and y are rounded, nothing else is.  Rows that start on 16-byte boundaries (pointers, and dim, ff, ldx times the element's size) take 16-byte loads; others are correct and slow.
+ * not touched.  bfloat16: the activation and y are rounded, nothing else is.  Fast where all rows of x and the matrices start on 16-byte boundaries
+ * (pointers, and dim, ff and ldx times the element's size), 1.1 to 1.5 times as long where they start on 4-byte ones, 8 times and more with bfloat16 rows that do not.
  * workspace: at least nl_op_experts_workspace bytes, on a 16-byte boundary, this call's alone until its work is done (two graphs that may
  * run at the same time need one each).  x and y must not overlap. */
 NL_API int nl_op_experts(int device, void *stream, const nl_experts_desc *d, int n, const void *x, int64_t ldx, const int32_t *ids,
@@ -77,7 +78,8 @@ NL_API int nl_op_residual_norm(int device, void *stream, const nl_residual_norm_
  * The layer's nl_layer_desc has ff == 0.  Tensors: norm2 (and norm2_post) as for a feed-forward, and
  *     layers.N.ff.router                       [experts, dim],  ff.router_bias [experts] with bias (sigmoid scores only, joins the choice alone)
  *     layers.N.ff.experts.gate / up            [experts * ff, dim], expert behind expert
- *     layers.N.ff.experts.down                 [experts * dim, ff] */
+ *     layers.N.ff.experts.down                 [experts * dim, ff]
+ * In bfloat16 a token's choice can differ between decode and prompt launches where two keys lie within the rounding of the router's operand. */
 typedef struct {
     int32_t experts, per_token, ff, act;        /* ff: width of an expert; act: NL_ACT_* */
     int32_t score, renorm, bias;                /* as in nl_route_desc */

@@ -328,9 +328,9 @@ template <bool SILU> __device__ __forceinline__ f32x4 activate(f32x4 gate, f32x4
     return v;
 }
 
-// Rows that do not start on 16-byte boundaries: 16 places x 32 rows of one expert by a workgroup, K dealt to its four wavefronts, elements one by one
-// straight to registers (about ten times as long as with 16-byte pieces).  FIRST: gate and up rows of the tokens -> h; else rows of down of h -> part
-// (32-bit: a third rounding to bfloat16, beside the activation's and the sum's, would make the error 1.2 times as large: 2.9e-3 instead of 2.4e-3).
+// Rows that do not even start on 4-byte boundaries (bfloat16): 16 places x 32 rows of one expert by a workgroup, K dealt to its four wavefronts, elements one
+// by one straight to registers.  FIRST: gate and up rows of the tokens -> h; else rows of down of h -> part (32-bit: a third rounding to bfloat16, beside
+// the activation's and the sum's, would make the error 1.2 times as large: 2.9e-3 instead of 2.4e-3).
 template <typename T, bool FIRST>
 __global__ void __launch_bounds__(256) experts_any_kernel(ExpertsParams P) {
     constexpr int R = 2, M = FIRST ? 2 : 1, N = R * M;
@@ -464,14 +464,14 @@ __global__ void __launch_bounds__(256) experts_token_second_kernel(ExpertsParams
     } else P.part[(long long)t * P.dim + row] = sum;
 }
 
-// Prompts: WR x WT wavefronts of RTW row tiles x NTW token tiles each; 128 bytes of every row at a time go through two LDS stages by LDS-DMA.  A
-// 1 KiB piece is 8 rows x 128 bytes, whole lines of the rows as they lie; in LDS the 16-byte run q of row r is at q ^ (r % 8), so that the 16 rows of a
-// fragment are read from all banks.  FIRST: row tiles alternate between gate and up.
+// Prompts: WR x WT wavefronts of RTW row tiles x NTW token tiles each; 128 bytes of every row at a time go through a ring of two or three LDS stages by
+// LDS-DMA, a piece of 8 rows (UNIT 16 bytes a lane), whole lines of the rows as they lie, or of 2 (UNIT 4, for rows that start on 4-byte boundaries only).  In
+// LDS the 16-byte run q of row r is at q ^ (r % 8), so that the 16 rows of a fragment are read from all banks.  FIRST: row tiles alternate between gate and up.
 // Workgroups b, b + 8, ... run on one XCD and take a contiguous range of (expert, row block, token tile): both operands of neighbours are in its L2.
-template <typename T, int RTW_, int NTW_, int WR_, int WT_, int NST_ = 2> struct Grouped {
-    static constexpr int NST = NST_, RTW = RTW_, NTW = NTW_, WR = WR_, WT = WT_, RT = WR * RTW, NT = WT * NTW, STAGE = (RT + NT) * 2048, LDS = NST * STAGE, NW = WR * WT, THREADS = 64 * NW,
-                         PW = STAGE / 1024 / NW, BT = NT * 16, KB = 128 / (int)sizeof(T), KK = KB / 32, PER_CU = 163840 / LDS;
-    static_assert(PW * NW * 1024 == STAGE, "pieces");
+template <typename T, int RTW_, int NTW_, int WR_, int WT_, int NST_ = 2, int UNIT_ = 16> struct Grouped {
+    static constexpr int NST = NST_, UNIT = UNIT_, PIECE = 64 * UNIT, RTW = RTW_, NTW = NTW_, WR = WR_, WT = WT_, RT = WR * RTW, NT = WT * NTW, STAGE = (RT + NT) * 2048, LDS = NST * STAGE, NW = WR * WT, THREADS = 64 * NW,
+                         PW = STAGE / PIECE / NW, BT = NT * 16, KB = 128 / (int)sizeof(T), KK = KB / 32, PER_CU = 163840 / LDS;
+    static_assert(PW * NW * PIECE == STAGE && NW * PIECE % 1024 == 0 && PW * (NST - 1) < 64, "pieces");
 };
 __device__ const f32x4 zero_piece = {0.f, 0.f, 0.f, 0.f};
 template <typename T> __device__ __forceinline__ Frag<T> swizzled_frag(const char *tile, int r, int g, int kk);
@@ -488,7 +488,7 @@ template <> __device__ __forceinline__ Frag<float> swizzled_frag<float>(const ch
 }
 template <typename T, bool FIRST, typename S>
 __global__ void __launch_bounds__(S::THREADS, S::NW * S::PER_CU / 4) experts_many_kernel(ExpertsParams P) {
-    constexpr int RT = S::RT, NST = S::NST, STAGE = S::STAGE, NW = S::NW, PW = S::PW, BT = S::BT, KB = S::KB, KK = S::KK, RTW = S::RTW, NTW = S::NTW;
+    constexpr int RT = S::RT, NST = S::NST, UNIT = S::UNIT, PIECE = S::PIECE, STAGE = S::STAGE, NW = S::NW, PW = S::PW, BT = S::BT, KB = S::KB, KK = S::KK, RTW = S::RTW, NTW = S::NTW;
     constexpr int BR = (FIRST ? RT / 2 : RT) * 16;        // output rows of the workgroup
     extern __shared__ __align__(16) char lds[];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15, wr = w % S::WR, wt = w / S::WR;
@@ -508,25 +508,30 @@ __global__ void __launch_bounds__(S::THREADS, S::NW * S::PER_CU / 4) experts_man
     };
     const int turn = rb * nks / nrb;                     // (row blocks start at different columns: their rows would else ask the same memory channels)
     const char *src[PW];
-    const int k0 = ((lane & 7) ^ (lane >> 3)) * (16 / (int)sizeof(T));
+    constexpr int LR = 128 / UNIT, PR = PIECE / 128;     // lanes of a row, rows of a piece
+    const int run = lane % LR * UNIT / 16 ^ (w * PR + lane / LR) % 8, k0 = (run * 16 + lane % LR * UNIT % 16) / (int)sizeof(T);      // (a wavefront's pieces are whole eights of rows apart)
     int there = NST == 2 ? 0 : PW;                       // pieces with a token or a row of the matrix: the first ones (all, where waits count them)
 #pragma unroll
     for (int i = 0; i < PW; i++) {
         const int u = i * NW + w;
-        if (NST == 2 && ((u >> 1) < RT || ((u >> 1) - RT) * 16 + (u & 1) * 8 < count)) there = i + 1;
-        src[i] = reinterpret_cast<const char *>(row_of(u >> 1, (u & 1) * 8 + (lane >> 3)) + k0);
+        if (NST == 2 && u * PR - RT * 16 < count) there = i + 1;
+        src[i] = reinterpret_cast<const char *>(row_of(u * PR >> 4, u * PR % 16 + lane / LR) + k0);
     }
+    auto bring = [&](const void *from, int st, int i) {
+        if constexpr (UNIT == 16) lds_dma16(from, lds + st * STAGE + (i * NW + w) * PIECE);
+        else lds_dma4(from, lds + st * STAGE + (i * NW + w) * PIECE);
+    };
     auto issue = [&](int ks, int st) {
         if ((ks += turn) >= nks) ks -= nks;
         if ((ks + 1) * KB <= K) {
 #pragma unroll
             for (int i = 0; i < PW; i++)
-                if (i < there) lds_dma16(src[i] + (long long)ks * 128, lds + st * STAGE + (i * NW + w) * 1024);
+                if (i < there) bring(src[i] + (long long)ks * 128, st, i);
         } else {                                         // (behind the row's end: zeros)
             const unsigned long long in = ks * KB + k0 < K ? ~0ull : 0, zero = reinterpret_cast<unsigned long long>(&zero_piece) & ~in;
 #pragma unroll
             for (int i = 0; i < PW; i++)
-                if (i < there) lds_dma16(reinterpret_cast<const char *>((reinterpret_cast<unsigned long long>(src[i] + (long long)ks * 128) & in) | zero), lds + st * STAGE + (i * NW + w) * 1024);
+                if (i < there) bring(reinterpret_cast<const char *>((reinterpret_cast<unsigned long long>(src[i] + (long long)ks * 128) & in) | zero), st, i);
         }
     };
     f32x4 acc[RTW][NTW] = {};

@@ -81,6 +81,11 @@ __device__ __forceinline__ void lds_dma16(const void *src_lane, void *lds_base) 
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src_lane,
                                      (__attribute__((address_space(3))) void *)lds_base, 16, 0, 0);
 }
+// 4 bytes per lane
+__device__ __forceinline__ void lds_dma4(const void *src_lane, void *lds_base) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src_lane,
+                                     (__attribute__((address_space(3))) void *)lds_base, 4, 0, 0);
+}
 // until at most N of this wavefront's vector memory operations are in flight (they complete in order)
 template <int N> __device__ __forceinline__ void vm_wait() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 

@@ -37,7 +37,7 @@ hipError_t start_lds(dim3 grid, dim3 block, size_t lds, hipStream_t st, A... arg
     return start(KERNEL, grid, block, lds, st, args...);
 }
 
-inline bool on16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+inline bool on(const void *p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
 }  // namespace
 
@@ -124,8 +124,10 @@ template <typename T, bool FIRST> static hipError_t grouped_product(const Expert
 }
 template <typename T> static hipError_t experts(const ExpertsParams &P, bool &summed, hipStream_t st) {
     const int slots = P.n * P.k;
-    constexpr int W = 16 / (int)sizeof(T);               // elements of a 16-byte piece
-    const bool vec = on16(P.x) && on16(P.gate) && on16(P.up) && on16(P.down) && P.ldx % W == 0 && P.dim % W == 0 && P.ff % W == 0;
+    auto rows_on = [&](size_t bytes) {                   // every row starts on such a boundary
+        return on(P.x, bytes) && on(P.gate, bytes) && on(P.up, bytes) && on(P.down, bytes) && P.ldx * sizeof(T) % bytes == 0 && P.dim * sizeof(T) % bytes == 0 && P.ff * sizeof(T) % bytes == 0;
+    };
+    const bool vec = rows_on(16);
     hipError_t rc;
     // Slot by slot where grouping hardly saves a matrix: one token, or half as many slots as experts (4 tokens to 8 of 64 of 1536 x 768 38 us, grouped 48;
     // 8 tokens 68 and 60.  2 tokens to 2 of 8 of 4096 x 11008 188 and 240, 4 tokens 349 and 280).
@@ -139,9 +141,19 @@ template <typename T> static hipError_t experts(const ExpertsParams &P, bool &su
         if ((rc = grouped_product<T, true>(P, st)) != hipSuccess) return rc;
         return grouped_product<T, false>(P, st);
     }
-    const int hit = std::min(P.experts, slots), tiles = std::min(hit + (slots - hit) / 16, 65535);
-    if ((rc = start(experts_any_kernel<T, true>, dim3((P.ff + 31) / 32, tiles), dim3(256), 0, st, P)) != hipSuccess) return rc;
-    return start(experts_any_kernel<T, false>, dim3((P.dim + 31) / 32, tiles), dim3(256), 0, st, P);
+    // us a pass with rows on 16-byte boundaries, on 4-byte and on 2-byte ones: 333 tokens to 2 of 8 of 768 x 2048 32, 41, 499; 64 to 6 of 64 of 1536 x 1024
+    // 119, 125, 958; 2047 to 8 of 64 of 1536 x 768 251, 364, 7743
+    if (rows_on(4)) {
+        using Any = Grouped<T, 2, sizeof(T) == 2 ? 2 : 1, 2, 2, 3, 4>;
+        if ((rc = grouped<T, true, Any>(P, st)) != hipSuccess) return rc;
+        return grouped<T, false, Any>(P, st);
+    }
+    if constexpr (sizeof(T) == 2) {
+        const int hit = std::min(P.experts, slots), tiles = std::min(hit + (slots - hit) / 16, 65535);
+        if ((rc = start(experts_any_kernel<T, true>, dim3((P.ff + 31) / 32, tiles), dim3(256), 0, st, P)) != hipSuccess) return rc;
+        return start(experts_any_kernel<T, false>, dim3((P.dim + 31) / 32, tiles), dim3(256), 0, st, P);
+    }
+    return hipErrorInvalidValue;                         // (the entry points refuse such pointers)
 }
 
 template <typename T> static hipError_t close(const CloseParams &P, hipStream_t st) {
@@ -259,9 +271,11 @@ int nl_op_experts(int device, void *stream, const nl_experts_desc *d, int n, con
     if (n == 0) return NL_OK;
     if (!x || !ids || !weights || !gate || !up || !down || !y || !workspace) return fail(NL_ERR_INVALID, "experts: null argument");
     if (ldx < d->dim || ldy < d->dim) return fail(NL_ERR_INVALID, "experts: ldx %lld and ldy %lld, rows have %d elements", (long long)ldx, (long long)ldy, d->dim);
+    const size_t size = d->dtype == NL_DTYPE_F32 ? 4 : 2;
+    if (!on(x, size) || !on(gate, size) || !on(up, size) || !on(down, size) || !on(y, size)) return fail(NL_ERR_INVALID, "experts: an array is not on a boundary of its elements");
     const ExpertsLayout L = experts_layout(n, d->per_token, d->experts, d->dim, d->ff, d->dtype);
     if (workspace_bytes < L.bytes) return fail(NL_ERR_INVALID, "experts: workspace of %llu bytes, %llu are needed", (unsigned long long)workspace_bytes, (unsigned long long)L.bytes);
-    if (!on16(workspace)) return fail(NL_ERR_INVALID, "experts: workspace is not on a 16-byte boundary");
+    if (!on(workspace, 16)) return fail(NL_ERR_INVALID, "experts: workspace is not on a 16-byte boundary");
     ExpertsParams P{};
     P.x = x; P.gate = gate; P.up = up; P.down = down; P.ldx = ldx; P.ids = ids; P.weights = weights; P.n = n; P.k = d->per_token; P.experts = d->experts;
     P.dim = d->dim; P.ff = d->ff; P.act = d->act;

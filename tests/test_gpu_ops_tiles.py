@@ -11,7 +11,7 @@ pytestmark = pytest.mark.gpu
 def skewed(n, E, k, seed=0):
     """Experts asked for very differently, and places without one."""
     rng = np.random.default_rng(seed)
-    ids = np.minimum(rng.geometric(3.0 / E, (n, k)) - 1, E + 1).astype(np.int32)      # E and E + 1 are no experts
+    ids = np.minimum(rng.geometric(3.0 / max(E, 3), (n, k)) - 1, E + 1).astype(np.int32)      # E and E + 1 are no experts
     ids[rng.random((n, k)) < 0.05] = -1
     return ids
 
@@ -76,3 +76,17 @@ def test_the_same_bits_every_time_with_every_tile():
             m.queue()
             sync()
             assert np.array_equal(first, m.y.bits())
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("n, dim, ff, E, k", [(1, 34, 18, 3, 2), (3, 2, 2, 2, 1), (40, 100, 50, 6, 2), (70, 62, 66, 3, 2), (70, 126, 130, 3, 1), (200, 90, 258, 2, 2), (333, 190, 102, 5, 2)])
+def test_rows_on_four_byte_boundaries(n, dim, ff, E, k, dtype):
+    Experts(n, dim, ff, E, k, dtype, seed=n).run()
+    Experts(n, dim, ff, E, k, dtype, seed=n, ids=skewed(n, E, k), x_apart=dim + 6, y_apart=dim + 1).run()
+    Experts(n, 64, 48, E, k, dtype, seed=n, shift=2, x_apart=66).run()
+
+
+@pytest.mark.parametrize("cols", [2, 30, 32, 34, 62, 64, 66, 94, 130, 190, 194, 258])
+def test_rows_that_end_within_a_four_byte_stage(cols):
+    Experts(70, cols, 66, 3, 2, "bfloat16", seed=cols).run()
+    Experts(70, 66, cols, 3, 2, "bfloat16", seed=cols).run()
