@@ -133,3 +133,16 @@ def test_refusals():
     assert up(b"layers.1.ff.router", 8, 64) == -1
     assert L.nl_finalize(h) < 0 and b"not uploaded" in L.nl_last_error(h)
     L.nl_destroy(h)
+
+
+@pytest.mark.parametrize("cfg", [MODELS["sigmoid_and_bias"][0], MODELS["norms_behind"][0]], ids=["Ganidra", "Pabalix"])
+def test_from_a_folder_through_the_scheduler(cfg, tmp_path):
+    from nanollama_amd import registry
+    from nanollama_amd.scheduler import Scheduler
+    w = weights(cfg, 6)
+    m = registry.load_model(ss.write_folder(str(tmp_path / "model"), cfg, w), max_streams=3, dtype="float32", seq_len=128)
+    prompts = [tokens(n, cfg["vocab"], seed=n) for n in (3, 17, 1, 40, 9)]
+    got = Scheduler(m).generate(prompts, 8)
+    want = [so.greedy(cfg, floats(w), p, 8) for p in prompts]
+    assert [[int(t) for t in g] for g in got] == want
+    m.close()
