@@ -467,6 +467,9 @@ __global__ void __launch_bounds__(256) experts_token_second_kernel(ExpertsParams
 // Prompts: WR x WT wavefronts of RTW row tiles x NTW token tiles each; 128 bytes of every row at a time go through a ring of two or three LDS stages by
 // LDS-DMA, a piece of 8 rows (UNIT 16 bytes a lane), whole lines of the rows as they lie, or of 2 (UNIT 4, for rows that start on 4-byte boundaries only).  In
 // LDS the 16-byte run q of row r is at q ^ (r % 8), so that the 16 rows of a fragment are read from all banks.  FIRST: row tiles alternate between gate and up.
+// Bound by what a CU's L1 has on its way: about 64 KB, 1.1 us each.  Two workgroups of 128 x 128 take 1.05 us a stage (43 KB/us of DMA, 1.0 PFLOP/s over the chip); as long
+// where nobody waits for a stage, 5 us less of 128 where LDS is not read, 48 less without the DMA; one of 256 x 256 1.8 us (1.2 PFLOP/s), half the
+// bytes a product, but as few and as large workgroups as leave CUs idle.  Tokens that fill a small part of a tile, and few rounds, cost more than either.
 // Workgroups b, b + 8, ... run on one XCD and take a contiguous range of (expert, row block, token tile): both operands of neighbours are in its L2.
 template <typename T, int RTW_, int NTW_, int WR_, int WT_, int NST_ = 2, int UNIT_ = 16> struct Grouped {
     static constexpr int NST = NST_, UNIT = UNIT_, PIECE = 64 * UNIT, RTW = RTW_, NTW = NTW_, WR = WR_, WT = WT_, RT = WR * RTW, NT = WT * NTW, STAGE = (RT + NT) * 2048, LDS = NST * STAGE, NW = WR * WT, THREADS = 64 * NW,
@@ -506,7 +509,9 @@ __global__ void __launch_bounds__(S::THREADS, S::NW * S::PER_CU / 4) experts_man
         const int place = first + min((t - RT) * 16 + r, count - 1);
         return FIRST ? reinterpret_cast<const T *>(P.x) + (long long)(P.order[place] / P.k) * P.ldx : reinterpret_cast<const T *>(P.h) + (long long)place * P.ff;
     };
-    const int turn = rb * nks / nrb;                     // (row blocks start at different columns: their rows would else ask the same memory channels)
+    // (XCDs start at different columns, and four row blocks in turn: 2047 tokens to 8 of 64 of 1536 x 768 126 / 85 us; all at the first one 126 / 87, every row
+    // block at its own 128 / 87, every token tile too 144 / 90; down of 4096 x 11008 374, 386, 448, 528)
+    const int turn = ((blockIdx.x & 7) * nks / 8 + (rb & 3)) % nks;
     const char *src[PW];
     constexpr int LR = 128 / UNIT, PR = PIECE / 128;     // lanes of a row, rows of a piece
     const int run = lane % LR * UNIT / 16 ^ (w * PR + lane / LR) % 8, k0 = (run * 16 + lane % LR * UNIT % 16) / (int)sizeof(T);      // (a wavefront's pieces are whole eights of rows apart)
