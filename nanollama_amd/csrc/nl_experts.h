@@ -501,44 +501,54 @@ __global__ void __launch_bounds__(S::THREADS, S::NW * S::PER_CU / 4) experts_man
     if ((int)(blockIdx.x >> 3) >= per || id >= all) return;
     const Group G = groups.find(id / nrb);
     const int tiles = (G.b - G.a + BT - 1) / BT, local = id - G.before * nrb, rb = local / tiles, first = G.a + (local - rb * tiles) * BT, count = min(BT, G.b - first);
-    auto row_of = [&](int t, int r) -> const T * {       // row r of tile t of a stage
-        if (t < RT) {
-            const T *W = reinterpret_cast<const T *>(!FIRST ? P.down : t & 1 ? P.up : P.gate);
-            return W + ((long long)G.e * rows + min(rb * BR + (FIRST ? t >> 1 : t) * 16 + r, rows - 1)) * K;
-        }
-        const int place = first + min((t - RT) * 16 + r, count - 1);
-        return FIRST ? reinterpret_cast<const T *>(P.x) + (long long)(P.order[place] / P.k) * P.ldx : reinterpret_cast<const T *>(P.h) + (long long)place * P.ff;
-    };
     // (XCDs start at different columns, and four row blocks in turn: 2047 tokens to 8 of 64 of 1536 x 768 126 / 85 us; all at the first one 126 / 87, every row
     // block at its own 128 / 87, every token tile too 144 / 90; down of 4096 x 11008 374, 386, 448, 528)
     const int turn = ((blockIdx.x & 7) * nks / 8 + (rb & 3)) % nks;
     const char *src[PW];
-    constexpr int LR = 128 / UNIT, PR = PIECE / 128;     // lanes of a row, rows of a piece
+    constexpr int LR = 128 / UNIT, PR = PIECE / 128, PA = RT * 16 / PR / NW;         // lanes of a row, rows of a piece, a wavefront's pieces of the matrix
+    static_assert(PA * NW * PR == RT * 16, "pieces of the matrix");
     const int run = lane % LR * UNIT / 16 ^ (w * PR + lane / LR) % 8, k0 = (run * 16 + lane % LR * UNIT % 16) / (int)sizeof(T);      // (a wavefront's pieces are whole eights of rows apart)
-    int there = NST == 2 ? 0 : PW;                       // pieces with a token or a row of the matrix: the first ones (all, where waits count them)
+    int there = NST == 2 ? PA : PW;                      // pieces with a token or a row of the matrix: the first ones (all, where waits count them)
+    int token[PW - PA];                                  // (asked for now, needed behind the matrix's first pieces)
 #pragma unroll
-    for (int i = 0; i < PW; i++) {
-        const int u = i * NW + w;
-        if (NST == 2 && u * PR - RT * 16 < count) there = i + 1;
-        src[i] = reinterpret_cast<const char *>(row_of(u * PR >> 4, u * PR % 16 + lane / LR) + k0);
+    for (int i = PA; i < PW; i++) {
+        const int at = (i * NW + w) * PR - RT * 16;
+        if (NST == 2 && at < count) there = i + 1;
+        const int place = first + min(at + lane / LR, count - 1);
+        token[i - PA] = FIRST ? P.order[place] : place;
+    }
+#pragma unroll
+    for (int i = 0; i < PA; i++) {
+        const int r = (i * NW + w) * PR + lane / LR, t = r >> 4;                      // row of the stage, its tile
+        const T *W = reinterpret_cast<const T *>(!FIRST ? P.down : t & 1 ? P.up : P.gate);
+        src[i] = reinterpret_cast<const char *>(W + ((long long)G.e * rows + min(rb * BR + (FIRST ? t >> 1 : t) * 16 + (r & 15), rows - 1)) * K + k0);
     }
     auto bring = [&](const void *from, int st, int i) {
         if constexpr (UNIT == 16) lds_dma16(from, lds + st * STAGE + (i * NW + w) * PIECE);
         else lds_dma4(from, lds + st * STAGE + (i * NW + w) * PIECE);
     };
-    auto issue = [&](int ks, int st) {
+    auto issue = [&](int ks, int st, auto from, auto to) {
+        constexpr int I0 = decltype(from)::value, I1 = decltype(to)::value;
         if ((ks += turn) >= nks) ks -= nks;
         if ((ks + 1) * KB <= K) {
 #pragma unroll
-            for (int i = 0; i < PW; i++)
-                if (i < there) bring(src[i] + (long long)ks * 128, st, i);
+            for (int i = I0; i < I1; i++)
+                if (i < PA || i < there) bring(src[i] + (long long)ks * 128, st, i);
         } else {                                         // (behind the row's end: zeros)
             const unsigned long long in = ks * KB + k0 < K ? ~0ull : 0, zero = reinterpret_cast<unsigned long long>(&zero_piece) & ~in;
 #pragma unroll
-            for (int i = 0; i < PW; i++)
-                if (i < there) bring(reinterpret_cast<const char *>((reinterpret_cast<unsigned long long>(src[i] + (long long)ks * 128) & in) | zero), st, i);
+            for (int i = I0; i < I1; i++)
+                if (i < PA || i < there) bring(reinterpret_cast<const char *>((reinterpret_cast<unsigned long long>(src[i] + (long long)ks * 128) & in) | zero), st, i);
         }
     };
+    using None = std::integral_constant<int, 0>;
+    using Some = std::integral_constant<int, PA>;
+    using Whole = std::integral_constant<int, PW>;
+    issue(0, 0, None(), Some());
+#pragma unroll
+    for (int i = PA; i < PW; i++)
+        src[i] = reinterpret_cast<const char *>((FIRST ? reinterpret_cast<const T *>(P.x) + (long long)(token[i - PA] / P.k) * P.ldx
+                                                       : reinterpret_cast<const T *>(P.h) + (long long)token[i - PA] * P.ff) + k0);
     f32x4 acc[RTW][NTW] = {};
     Frag<T> fa[KK][RTW], fb[KK][NTW];
     const bool busy = wt * NTW * 16 < count;             // (wavefronts without a token only bring pieces)
@@ -568,12 +578,13 @@ __global__ void __launch_bounds__(S::THREADS, S::NW * S::PER_CU / 4) experts_man
         else vm_wait<0>();
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if (s - 1 + NST < nks) issue(s - 1 + NST, st);
+        if (s - 1 + NST < nks) issue(s - 1 + NST, st, None(), Whole());
         st = st + 1 == NST ? 0 : st + 1;
     };
+    issue(0, 0, Some(), Whole());
 #pragma unroll
-    for (int s = 0; s < NST; s++)
-        if (s < nks) issue(s, s);
+    for (int s = 1; s < NST; s++)
+        if (s < nks) issue(s, s, None(), Whole());
     if (nks >= NST && there == PW) vm_wait<PW *(NST - 1)>();
     else vm_wait<0>();
     lds_barrier();
