@@ -369,9 +369,23 @@ __global__ void __launch_bounds__(256) experts_any_kernel(ExpertsParams P) {
     }
 }
 
+// V consecutive elements as floats
+template <int V> __device__ __forceinline__ void load_vec(const float *p, float *v) {
+    if constexpr (V == 4) *reinterpret_cast<f32x4 *>(v) = *reinterpret_cast<const f32x4 *>(p);
+    else v[0] = *p;
+}
+template <int V> __device__ __forceinline__ void load_vec(const bf16 *p, float *v) {
+    if constexpr (V == 4) {
+        const bf16x4 b = *reinterpret_cast<const bf16x4 *>(p);
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = (float)b[i];
+    } else v[0] = (float)*p;
+}
+
 // A few tokens: no grouping, no matrix instructions; a row of a matrix is read by a whole wavefront in 16-byte pieces, one row for every slot that
-// asks for it.  First the activations of slot blockIdx.y (h is by slot here), then rows of the sum over token blockIdx.y's slots: a lane keeps its share
-// of all of them, one sum over the wavefront at the end.
+// asks for it.  First the activations of slot blockIdx.y (h is by slot here, and 32-bit: no matrix instruction wants them rounded, and rounded ones make the
+// error 1.4 times as large, by chance 1.6 times for a single token), then rows of the sum over token blockIdx.y's slots: a lane keeps its share of all of
+// them, one sum over the wavefront at the end.
 template <typename T> struct Piece { static constexpr int N = 16 / (int)sizeof(T); T v[N]; };
 template <typename T> __device__ __forceinline__ Piece<T> load_piece(const T *p) {
     Piece<T> r;
@@ -420,7 +434,7 @@ __global__ void __launch_bounds__(256) experts_token_first_kernel(ExpertsParams 
     else if (P.dim > k0) some(k0, std::integral_constant<int, 1>());
     ga = wave_sum(ga);
     ub = wave_sum(ub);
-    if (lane == 0) put(reinterpret_cast<T *>(P.h) + (long long)slot * P.ff + row, ga * sigmoid_f32(P.act == NL_ACT_SILU ? ga : gelu_arg(ga)) * ub);
+    if (lane == 0) reinterpret_cast<float *>(P.h)[(long long)slot * P.ff + row] = ga * sigmoid_f32(P.act == NL_ACT_SILU ? ga : gelu_arg(ga)) * ub;
 }
 template <typename T>
 __global__ void __launch_bounds__(256) experts_token_second_kernel(ExpertsParams P) {
@@ -433,18 +447,23 @@ __global__ void __launch_bounds__(256) experts_token_second_kernel(ExpertsParams
     auto some = [&](int j0, int k, auto count) {         // `count` slots from the j0-th on, a piece each
         constexpr int C = decltype(count)::value;
         const int kc = k < P.ff ? k : 0;
-        Piece<T> hv[C], dv[C];
+        Piece<T> dv[C];
+        float hv[C][N];
 #pragma unroll
         for (int i = 0; i < C; i++) {
             const int j = min(j0 + i, P.k - 1), e = __builtin_amdgcn_readlane(id, j), ec = e >= 0 && e < P.experts ? e : 0;
             dv[i] = load_piece(reinterpret_cast<const T *>(P.down) + ((long long)ec * P.dim + row) * P.ff + kc);
-            hv[i] = load_piece(reinterpret_cast<const T *>(P.h) + (long long)(t * P.k + j) * P.ff + kc);
+#pragma unroll
+            for (int p = 0; p < N; p += 4) load_vec<4>(reinterpret_cast<const float *>(P.h) + (long long)(t * P.k + j) * P.ff + kc + p, hv[i] + p);
         }
 #pragma unroll
         for (int i = 0; i < C; i++) {
             const int j = min(j0 + i, P.k - 1), e = __builtin_amdgcn_readlane(id, j);
             const bool in = j0 + i < P.k && e >= 0 && e < P.experts && k < P.ff;
-            const float v = dot_piece(dv[i], hv[i]) * lane_value(weight, j);
+            float v = 0.f;
+#pragma unroll
+            for (int p = 0; p < N; p++) v = fmaf((float)dv[i].v[p], hv[i][p], v);
+            v *= lane_value(weight, j);
             sum += in ? v : 0.f;
         }
     };
@@ -650,18 +669,6 @@ template <typename T> __device__ __forceinline__ float close_value(const ClosePa
             if (id >= 0 && id < P.experts) v += P.part[s * P.dim + k];
         }
     return v;
-}
-// V consecutive elements as floats
-template <int V> __device__ __forceinline__ void load_vec(const float *p, float *v) {
-    if constexpr (V == 4) *reinterpret_cast<f32x4 *>(v) = *reinterpret_cast<const f32x4 *>(p);
-    else v[0] = *p;
-}
-template <int V> __device__ __forceinline__ void load_vec(const bf16 *p, float *v) {
-    if constexpr (V == 4) {
-        const bf16x4 b = *reinterpret_cast<const bf16x4 *>(p);
-#pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = (float)b[i];
-    } else v[0] = (float)*p;
 }
 template <int V, typename T> __device__ __forceinline__ void store_vec(T *p, const float *v) {
     if constexpr (V == 4) put4(p, *reinterpret_cast<const f32x4 *>(v));

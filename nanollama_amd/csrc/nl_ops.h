@@ -26,7 +26,7 @@ struct ExpertsParams {
     int n, k, experts, dim, ff, act;      // act: NL_ACT_*
     // workspace (experts_layout)
     int *offs, *order;                    // first place of every expert [experts + 1]; place -> slot (token * k + j)
-    void *h;                              // [place][ff] activations
+    void *h;                              // [place][ff] activations in the element type, or [slot][ff] in 32 bits
     float *part;                          // [slot][dim] weighted results
     // launch_experts has these: where the sums of a few tokens go at once, if anywhere
     void *y;

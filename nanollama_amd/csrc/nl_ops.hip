@@ -53,6 +53,9 @@ hipError_t launch_route(const RouteParams &P, hipStream_t st) {
     return start(route_kernel<16>, grid, block, 0, st, P);
 }
 
+// Slot by slot where grouping hardly saves a matrix: one token, or half as many slots as experts (4 tokens to 8 of 64 of 1536 x 768 38 us, grouped 48;
+// 8 tokens 68 and 60.  2 tokens to 2 of 8 of 4096 x 11008 188 and 240, 4 tokens 349 and 280).
+inline size_t most_by_token(int k, int experts) { return std::max(k, experts / 2); }
 ExpertsLayout experts_layout(int n, int k, int experts, int dim, int ff, int dtype) {
     const size_t slots = (size_t)n * k, es = dtype == NL_DTYPE_F32 ? 4 : 2;
     auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
@@ -60,7 +63,7 @@ ExpertsLayout experts_layout(int n, int k, int experts, int dim, int ff, int dty
     L.offs = 0;
     L.order = up((size_t)(experts + 1) * 4);
     L.h = L.order + up(slots * 4);
-    L.part = L.h + up(slots * ff * es);
+    L.part = L.h + up(std::max(slots * es, std::min(slots, most_by_token(k, experts)) * 4) * ff);
     L.bytes = L.part + up(slots * dim * 4);
     return L;
 }
@@ -129,9 +132,7 @@ template <typename T> static hipError_t experts(const ExpertsParams &P, bool &su
     };
     const bool vec = rows_on(16);
     hipError_t rc;
-    // Slot by slot where grouping hardly saves a matrix: one token, or half as many slots as experts (4 tokens to 8 of 64 of 1536 x 768 38 us, grouped 48;
-    // 8 tokens 68 and 60.  2 tokens to 2 of 8 of 4096 x 11008 188 and 240, 4 tokens 349 and 280).
-    summed = vec && (P.n == 1 || 2ll * slots <= P.experts);
+    summed = vec && (size_t)slots <= most_by_token(P.k, P.experts);
     if (summed) {
         if ((rc = start(experts_token_first_kernel<T>, dim3((P.ff + 3) / 4, slots), dim3(256), 0, st, P)) != hipSuccess) return rc;
         return start(experts_token_second_kernel<T>, dim3((P.dim + 3) / 4, P.n), dim3(256), 0, st, P);
