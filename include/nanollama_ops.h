@@ -52,7 +52,8 @@ typedef struct {
 } nl_experts_desc;
 /* x [n][ldx], ids and weights [n][per_token], gate and up [experts][ff][dim], down [experts][dim][ff], y [n][ldy].  An id outside
  * [0, experts) adds nothing, whatever its weight (a row without any: y = 0); an id twice in a row counts twice.  Rows of y behind n are
- * not touched.  bfloat16: the activation (not of a few tokens) and y are rounded, nothing else is.  Fast where all rows of x and the matrices start on 16-byte boundaries
+ * not touched.  bfloat16: y is rounded, and the activation where more than 8 tokens come to an expert on the average or rows are
+ * not on 16-byte boundaries; nothing else is.  Fast where all rows of x and the matrices start on 16-byte boundaries
  * (pointers, and dim, ff and ldx times the element's size), 1.1 to 1.5 times as long where they start on 4-byte ones, 8 times and more with bfloat16 rows that do not.
  * workspace: at least nl_op_experts_workspace bytes, on a 16-byte boundary, this call's alone until its work is done (two graphs that may
  * run at the same time need one each).  x and y must not overlap. */

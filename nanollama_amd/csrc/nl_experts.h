@@ -490,8 +490,9 @@ __global__ void __launch_bounds__(256) experts_token_second_kernel(ExpertsParams
 // where nobody waits for a stage, 5 us less of 128 where LDS is not read, 48 less without the DMA; one of 256 x 256 1.8 us (1.2 PFLOP/s), half the
 // bytes a product, but as few and as large workgroups as leave CUs idle.  Tokens that fill a small part of a tile, and few rounds, cost more than either.
 // Workgroups b, b + 8, ... run on one XCD and take a contiguous range of (expert, row block, token tile): both operands of neighbours are in its L2.
-template <typename T, int RTW_, int NTW_, int WR_, int WT_, int NST_ = 2, int UNIT_ = 16> struct Grouped {
-    static constexpr int NST = NST_, UNIT = UNIT_, PIECE = 64 * UNIT, RTW = RTW_, NTW = NTW_, WR = WR_, WT = WT_, RT = WR * RTW, NT = WT * NTW, STAGE = (RT + NT) * 2048, LDS = NST * STAGE, NW = WR * WT, THREADS = 64 * NW,
+template <typename T, int RTW_, int NTW_, int WR_, int WT_, int NST_ = 2, int UNIT_ = 16, bool PAIR_ = false> struct Grouped {
+    static constexpr bool PAIR = PAIR_;
+    static constexpr int NST = NST_, UNIT = UNIT_, PIECE = 64 * UNIT, RTW = RTW_, NTW = NTW_, WR = WR_, WT = WT_, RT = WR * RTW, NT = WT * NTW, STAGE = (RT + (PAIR ? 2 : 1) * NT) * 2048, LDS = NST * STAGE, NW = WR * WT, THREADS = 64 * NW,
                          PW = STAGE / PIECE / NW, BT = NT * 16, KB = 128 / (int)sizeof(T), KK = KB / 32, PER_CU = 163840 / LDS;
     static_assert(PW * NW * PIECE == STAGE && NW * PIECE % 1024 == 0 && PW * (NST - 1) < 64, "pieces");
 };
@@ -512,6 +513,7 @@ template <typename T, bool FIRST, typename S>
 __global__ void __launch_bounds__(S::THREADS, S::NW * S::PER_CU / 4) experts_many_kernel(ExpertsParams P) {
     constexpr int RT = S::RT, NST = S::NST, UNIT = S::UNIT, PIECE = S::PIECE, STAGE = S::STAGE, NW = S::NW, PW = S::PW, BT = S::BT, KB = S::KB, KK = S::KK, RTW = S::RTW, NTW = S::NTW;
     constexpr int BR = (FIRST ? RT / 2 : RT) * 16;        // output rows of the workgroup
+    static_assert(!FIRST || !S::PAIR, "pairs are the activations'");
     extern __shared__ __align__(16) char lds[];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15, wr = w % S::WR, wt = w / S::WR;
     const int rows = FIRST ? P.ff : P.dim, K = FIRST ? P.dim : P.ff, nrb = (rows + BR - 1) / BR, nks = (K + KB - 1) / KB;
@@ -527,13 +529,13 @@ __global__ void __launch_bounds__(S::THREADS, S::NW * S::PER_CU / 4) experts_man
     constexpr int LR = 128 / UNIT, PR = PIECE / 128, PA = RT * 16 / PR / NW;         // lanes of a row, rows of a piece, a wavefront's pieces of the matrix
     static_assert(PA * NW * PR == RT * 16, "pieces of the matrix");
     const int run = lane % LR * UNIT / 16 ^ (w * PR + lane / LR) % 8, k0 = (run * 16 + lane % LR * UNIT % 16) / (int)sizeof(T);      // (a wavefront's pieces are whole eights of rows apart)
-    int there = NST == 2 ? PA : PW;                      // pieces with a token or a row of the matrix: the first ones (all, where waits count them)
+    int there = NST == 2 && !S::PAIR ? PA : PW;          // pieces with a token or a row of the matrix: the first ones (all, where waits count them)
     int token[PW - PA];                                  // (asked for now, needed behind the matrix's first pieces)
 #pragma unroll
     for (int i = PA; i < PW; i++) {
-        const int at = (i * NW + w) * PR - RT * 16;
-        if (NST == 2 && at < count) there = i + 1;
-        const int place = first + min(at + lane / LR, count - 1);
+        const int at = (i * NW + w) * PR - RT * 16;      // PAIR: the tokens' activations, then what is left of them
+        if (NST == 2 && !S::PAIR && at < count) there = i + 1;
+        const int place = first + min((S::PAIR ? at % (S::NT * 16) : at) + lane / LR, count - 1);
         token[i - PA] = FIRST ? P.order[place] : place;
     }
 #pragma unroll
@@ -567,14 +569,15 @@ __global__ void __launch_bounds__(S::THREADS, S::NW * S::PER_CU / 4) experts_man
 #pragma unroll
     for (int i = PA; i < PW; i++)
         src[i] = reinterpret_cast<const char *>((FIRST ? reinterpret_cast<const T *>(P.x) + (long long)(token[i - PA] / P.k) * P.ldx
-                                                       : reinterpret_cast<const T *>(P.h) + (long long)token[i - PA] * P.ff) + k0);
+                                                       : reinterpret_cast<const T *>(S::PAIR && (i * NW + w) * PR >= (RT + S::NT) * 16 ? P.h_rest : P.h) + (long long)token[i - PA] * P.ff) + k0);
     f32x4 acc[RTW][NTW] = {};
-    Frag<T> fa[KK][RTW], fb[KK][NTW];
+    constexpr int NF = S::PAIR ? 2 * NTW : NTW;
+    Frag<T> fa[KK][RTW], fb[KK][NF];
     const bool busy = wt * NTW * 16 < count;             // (wavefronts without a token only bring pieces)
     auto read = [&](int st, int kk, Frag<T> *a, Frag<T> *b) {
         const char *base = lds + st * STAGE;
 #pragma unroll
-        for (int t = 0; t < NTW; t++) b[t] = swizzled_frag<T>(base + (RT + wt * NTW + t) * 2048, c, g, kk);
+        for (int t = 0; t < NF; t++) b[t] = swizzled_frag<T>(base + (RT + wt * NTW + (t < NTW ? t : S::NT + t - NTW)) * 2048, c, g, kk);
 #pragma unroll
         for (int r = 0; r < RTW; r++) a[r] = swizzled_frag<T>(base + (wr * RTW + r) * 2048, c, g, kk);
     };
@@ -585,7 +588,10 @@ __global__ void __launch_bounds__(S::THREADS, S::NW * S::PER_CU / 4) experts_man
 #pragma unroll
             for (int r = 0; r < RTW; r++)                // (32 bits: a stage's 32 products by themselves, then into the sum: one chain over the row is off by twice as much)
                 if constexpr (sizeof(T) == 4) acc[r][t] += mma(a[r], b[t], f32x4{});
-                else acc[r][t] = mma(a[r], b[t], acc[r][t]);
+                else {
+                    acc[r][t] = mma(a[r], b[t], acc[r][t]);
+                    if constexpr (S::PAIR) acc[r][t] = mma(a[r], b[NTW + t], acc[r][t]);
+                }
         }
     };
     // (builtins, not lds_barrier(): the compiler has to know that nothing is on its way from LDS, or it waits for the next fragments before it
@@ -644,8 +650,19 @@ __global__ void __launch_bounds__(S::THREADS, S::NW * S::PER_CU / 4) experts_man
         if constexpr (FIRST) {
             T *h = reinterpret_cast<T *>(P.h) + (long long)place * P.ff;
 #pragma unroll
-            for (int r = 0; r < RTW; r += 2)
-                put_rows(h, rb * BR + (wr * RTW + r) * 8 + 4 * g, P.ff, P.act == NL_ACT_SILU ? activate<true>(acc[r][t], acc[r + 1][t]) : activate<false>(acc[r][t], acc[r + 1][t]));
+            for (int r = 0; r < RTW; r += 2) {
+                const f32x4 v = P.act == NL_ACT_SILU ? activate<true>(acc[r][t], acc[r + 1][t]) : activate<false>(acc[r][t], acc[r + 1][t]);
+                put_rows(h, rb * BR + (wr * RTW + r) * 8 + 4 * g, P.ff, v);
+                if (sizeof(T) == 2 && P.h_rest) {        // (not finite: nothing is left)
+                    f32x4 rest;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float d = v[i] - (float)(T)v[i];
+                        rest[i] = d - d == 0.f ? d : 0.f;
+                    }
+                    put_rows(reinterpret_cast<T *>(P.h_rest) + (long long)place * P.ff, rb * BR + (wr * RTW + r) * 8 + 4 * g, P.ff, rest);
+                }
+            }
         } else {
             const int slot = P.order[place];
             float *o = P.part + (long long)slot * P.dim;

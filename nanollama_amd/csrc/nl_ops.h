@@ -27,6 +27,7 @@ struct ExpertsParams {
     // workspace (experts_layout)
     int *offs, *order;                    // first place of every expert [experts + 1]; place -> slot (token * k + j)
     void *h;                              // [place][ff] activations in the element type, or [slot][ff] in 32 bits
+    void *h_rest;                         // [place][ff] what their rounding left, in the element type, or null; launch_experts has it
     float *part;                          // [slot][dim] weighted results
     // launch_experts has these: where the sums of a few tokens go at once, if anywhere
     void *y;

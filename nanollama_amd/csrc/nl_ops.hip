@@ -56,6 +56,10 @@ hipError_t launch_route(const RouteParams &P, hipStream_t st) {
 // Slot by slot where grouping hardly saves a matrix: one token, or half as many slots as experts (4 tokens to 8 of 64 of 1536 x 768 38 us, grouped 48;
 // 8 tokens 68 and 60.  2 tokens to 2 of 8 of 4096 x 11008 188 and 240, 4 tokens 349 and 280).
 inline size_t most_by_token(int k, int experts) { return std::max(k, experts / 2); }
+// Up to so many tokens an expert on the average bfloat16 activations go on as pairs (what rounding leaves beside what it makes): the weights' way from memory hides
+// the second product.  us of it without and with: 64 experts of 1536 x 768, 4 tokens each 25 and 27, 16 each 31 and 37; 6 each of 1536 x 1024 33 and 35; 8 of 4096 x
+// 11008, 4 each 112 and 115, 16 each 139 and 171.  Error against 64 bits 2.35e-3 and 1.66e-3, which is the result's own rounding.
+constexpr size_t PAIR_TOKENS = 8;
 ExpertsLayout experts_layout(int n, int k, int experts, int dim, int ff, int dtype) {
     const size_t slots = (size_t)n * k, es = dtype == NL_DTYPE_F32 ? 4 : 2;
     auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
@@ -63,7 +67,7 @@ ExpertsLayout experts_layout(int n, int k, int experts, int dim, int ff, int dty
     L.offs = 0;
     L.order = up((size_t)(experts + 1) * 4);
     L.h = L.order + up(slots * 4);
-    L.part = L.h + up(std::max(slots * es, std::min(slots, most_by_token(k, experts)) * 4) * ff);
+    L.part = L.h + up(std::max(slots * es, std::min(slots, std::max(most_by_token(k, experts), PAIR_TOKENS * experts)) * 4) * ff);
     L.bytes = L.part + up(slots * dim * 4);
     return L;
 }
@@ -125,7 +129,8 @@ template <typename T, bool FIRST> static hipError_t grouped_product(const Expert
     }
     return grouped<T, FIRST, Small>(P, st);
 }
-template <typename T> static hipError_t experts(const ExpertsParams &P, bool &summed, hipStream_t st) {
+template <typename T> static hipError_t experts(ExpertsParams P, bool &summed, hipStream_t st) {
+    P.h_rest = nullptr;
     const int slots = P.n * P.k;
     auto rows_on = [&](size_t bytes) {                   // every row starts on such a boundary
         return on(P.x, bytes) && on(P.gate, bytes) && on(P.up, bytes) && on(P.down, bytes) && P.ldx * sizeof(T) % bytes == 0 && P.dim * sizeof(T) % bytes == 0 && P.ff * sizeof(T) % bytes == 0;
@@ -139,7 +144,14 @@ template <typename T> static hipError_t experts(const ExpertsParams &P, bool &su
     }
     if ((rc = start(plan_kernel, dim3(P.experts), dim3(1024), 0, st, P.ids, slots, P.experts, P.offs, P.order)) != hipSuccess) return rc;
     if (vec) {
+        const bool pair = sizeof(T) == 2 && (size_t)slots <= PAIR_TOKENS * P.experts;
+        if (pair) P.h_rest = reinterpret_cast<T *>(P.h) + (size_t)slots * P.ff;
         if ((rc = grouped_product<T, true>(P, st)) != hipSuccess) return rc;
+        if constexpr (sizeof(T) == 2) if (pair) {
+            using Small = Grouped<T, 2, 1, 2, 2, 3, 16, true>;
+            using Low = Grouped<T, 4, 1, 2, 2, 2, 16, true>;
+            return grouped_us<false, Low>(P, 5.4, 2.9) < grouped_us<false, Small>(P, 5.4, 2.9) ? grouped<T, false, Low>(P, st) : grouped<T, false, Small>(P, st);
+        }
         return grouped_product<T, false>(P, st);
     }
     // us a pass with rows on 16-byte boundaries, on 4-byte and on 2-byte ones: 333 tokens to 2 of 8 of 768 x 2048 32, 41, 499; 64 to 6 of 64 of 1536 x 1024

@@ -2,6 +2,7 @@
 import numpy as np
 import pytest
 
+import ops_reference as ref
 from hip_arrays import Stream, sync
 from test_gpu_ops import Experts
 
@@ -90,3 +91,30 @@ def test_rows_on_four_byte_boundaries(n, dim, ff, E, k, dtype):
 def test_rows_that_end_within_a_four_byte_stage(cols):
     Experts(70, cols, 66, 3, 2, "bfloat16", seed=cols).run()
     Experts(70, 66, cols, 3, 2, "bfloat16", seed=cols).run()
+
+
+# slot by slot and activations as pairs: nothing but the result is rounded to bfloat16.  What is left of a rounded activation is at most 2^-8 of it, and that
+# is rounded by 2^-8 once more: 2^-16 of the activation; a result is off by half a step of its own beside that.
+@pytest.mark.parametrize("n, dim, ff, E, k", [(1, 768, 512, 64, 8), (4, 264, 136, 64, 8), (9, 264, 200, 12, 3), (32, 768, 512, 64, 8), (64, 520, 264, 32, 4), (31, 136, 1032, 8, 2), (128, 264, 776, 128, 8), (33, 64, 72, 300, 32)])
+def test_few_tokens_an_expert_keep_their_activations(n, dim, ff, E, k):
+    for ids in (None, skewed(n, E, k)):
+        m = Experts(n, dim, ff, E, k, "bfloat16", seed=n, ids=ids)
+        m.queue()
+        sync()
+        want, bound = ref.experts(m.x, m.ids, m.w, m.gate, m.up, m.down, "silu", 2.0 ** -16)
+        step = 2.0 ** (np.floor(np.log2(np.maximum(np.abs(want) + bound, 1e-30))) - 7)
+        assert np.all(np.abs(m.y.numpy() - want) <= step / 2 + bound)
+        assert m.y.untouched() and m.ws.untouched()
+
+
+def test_activations_that_are_no_numbers_stay_with_their_tokens():
+    for n in (1, 20, 200):
+        m = Experts(n, 64, 40, 8, 2, "bfloat16", seed=n)
+        m.x[0] = 1e38                                      # products past the largest number, in one token
+        m.dx.write(m.x)
+        m.queue()
+        sync()
+        got = m.y.numpy()
+        assert not np.all(np.isfinite(got[0])) and np.all(np.isfinite(got[1:]))
+        want, bound = ref.experts(m.x[1:], m.ids[1:], m.w[1:], m.gate, m.up, m.down, "silu", 2.0 ** -8)
+        assert np.all(np.abs(got[1:] - want) <= bound)
