@@ -118,3 +118,26 @@ def test_activations_that_are_no_numbers_stay_with_their_tokens():
         assert not np.all(np.isfinite(got[0])) and np.all(np.isfinite(got[1:]))
         want, bound = ref.experts(m.x[1:], m.ids[1:], m.w[1:], m.gate, m.up, m.down, "silu", 2.0 ** -8)
         assert np.all(np.abs(got[1:] - want) <= bound)
+
+
+def test_two_threads_at_once():
+    import threading
+    cases = [Experts(33, 264, 136, 8, 2, "bfloat16", seed=1), Experts(300, 136, 264, 8, 2, "bfloat16", seed=2), Experts(2, 264, 136, 16, 4, "bfloat16", seed=3)]
+    failed = []
+
+    def work(m):
+        try:
+            s = Stream()
+            for _ in range(50):
+                m.queue(s.number)
+            s.sync()
+            m.check()
+        except BaseException as e:      # noqa: B036 (told by the thread that asks)
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(m,)) for m in cases]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
