@@ -68,7 +68,14 @@ def test_no_tokens_is_no_work():
 
 def test_workspace_sizes():
     size = ops.experts_workspace(7, 3, 5, 40, 24)
-    assert size >= 7 * 3 * (40 * 4 + 24 * 2) + 6 * 4 + 21 * 4 and ops.experts_workspace(7, 3, 5, 40, 24, "float32") > size
+    assert size >= 7 * 3 * (40 * 4 + 24 * 2) + 6 * 4 + 21 * 4
+    # activations of few tokens an expert take as much in either type, those of many half as much in bfloat16
+    assert ops.experts_workspace(7, 3, 5, 40, 24, "float32") >= size
+    assert ops.experts_workspace(700, 3, 5, 40, 24, "float32") >= ops.experts_workspace(700, 3, 5, 40, 24) + 2000 * 24 * 2
+    # a workspace for n tokens serves fewer
+    for dtype in ("bfloat16", "float32"):
+        sizes = [ops.experts_workspace(n, 3, 50, 40, 24, dtype) for n in range(400)]
+        assert sizes == sorted(sizes)
     assert ops.experts_workspace(0, 3, 5, 40, 24) > 0
     with pytest.raises(_lib.NlError, match="per_token"):
         ops.experts_workspace(7, 0, 5, 40, 24)
