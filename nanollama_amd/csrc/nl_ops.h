@@ -61,6 +61,6 @@ struct CloseParams {
 };
 hipError_t launch_close(const CloseParams &P, int dtype, hipStream_t st);
 // the experts' products of P's tokens and the close C of their sums (its part, ids, k, experts, n and dim are filled in, base and d stay null)
-hipError_t launch_experts(ExpertsParams P, CloseParams C, int dtype, hipStream_t st);
+hipError_t launch_experts(const ExpertsParams &P, const CloseParams &C, int dtype, hipStream_t st);
 
 }  // namespace nl

@@ -38,12 +38,19 @@ hipError_t start_lds(dim3 grid, dim3 block, size_t lds, hipStream_t st, A... arg
 }
 
 inline bool on(const void *p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+template <typename T> inline T *behind(T *p, long long elements) { return p ? p + elements : p; }
+inline const void *behind(const void *p, long long elements, size_t size) { return behind(reinterpret_cast<const char *>(p), elements * (long long)size); }
+inline void *behind(void *p, long long elements, size_t size) { return behind(reinterpret_cast<char *>(p), elements * (long long)size); }
+
+// A launch's threads are counted in 32 bits, silently: 2^24 rows at a workgroup of 256 each return without an error and leave nearly all of them unwritten.
+// So many tokens go at once, others behind them.
+constexpr int CLOSE_TOKENS = 1 << 23, ROUTE_TOKENS = 1 << 25;
 
 }  // namespace
 
 namespace nl {
 
-hipError_t launch_route(const RouteParams &P, hipStream_t st) {
+static hipError_t route(const RouteParams &P, hipStream_t st) {
     const dim3 grid((P.n + 3) / 4), block(256);
     const int ne = (P.experts + 63) / 64;
     if (ne <= 1) return start(route_kernel<1>, grid, block, 0, st, P);
@@ -51,6 +58,16 @@ hipError_t launch_route(const RouteParams &P, hipStream_t st) {
     if (ne <= 4) return start(route_kernel<4>, grid, block, 0, st, P);
     if (ne <= 8) return start(route_kernel<8>, grid, block, 0, st, P);
     return start(route_kernel<16>, grid, block, 0, st, P);
+}
+hipError_t launch_route(const RouteParams &P, hipStream_t st) {
+    hipError_t rc = hipSuccess;
+    for (long long t = 0; t < P.n && rc == hipSuccess; t += ROUTE_TOKENS) {
+        RouteParams Q = P;
+        Q.n = (int)std::min<long long>(P.n - t, ROUTE_TOKENS);
+        Q.logits = behind(P.logits, t * P.ld); Q.ids = behind(P.ids, t * P.k); Q.weights = behind(P.weights, t * P.k);
+        rc = route(Q, st);
+    }
+    return rc;
 }
 
 // Slot by slot where grouping hardly saves a matrix: one token, or half as many slots as experts (4 tokens to 8 of 64 of 1536 x 768 38 us, grouped 48;
@@ -79,12 +96,31 @@ void place_experts(ExpertsParams &P, void *workspace, const ExpertsLayout &L) {
     P.part = reinterpret_cast<float *>(ws + L.part);
 }
 
-// One product of the experts with tiles of S.
-template <typename T, bool FIRST, typename S> static hipError_t grouped(const ExpertsParams &P, hipStream_t st) {
+// One product of the experts with tiles of S.  The most workgroups that it can need: an expert's last tile may hold one token.
+template <bool FIRST, typename S> static long long workgroups(const ExpertsParams &P) {
     const int slots = P.n * P.k, hit = std::min(P.experts, slots), rows = FIRST ? P.ff : P.dim, br = S::RT * (FIRST ? 8 : 16);
-    const long long most = ((hit + (slots - hit) / S::BT) * (long long)((rows + br - 1) / br) + 7) / 8 * 8;
-    if (most > INT_MAX / S::THREADS) return hipErrorInvalidConfiguration;
-    return start_lds<experts_many_kernel<T, FIRST, S>>(dim3((unsigned)most), dim3(S::THREADS), S::LDS, st, P);
+    return ((hit + (slots - hit) / S::BT) * (long long)((rows + br - 1) / br) + 7) / 8 * 8;
+}
+template <typename T, bool FIRST, typename S> static hipError_t grouped(const ExpertsParams &P, hipStream_t st) {
+    return start_lds<experts_many_kernel<T, FIRST, S>>(dim3((unsigned)workgroups<FIRST, S>(P)), dim3(S::THREADS), S::LDS, st, P);
+}
+// The tiles, rows x tokens.  32 bits: 64 x 32.  bfloat16: 64 x 64, 128 x 64, 128 x 128, 256 x 256; of activations in pairs 64 x 32 and 128 x 32.
+template <typename T> using Small = Grouped<T, 2, sizeof(T) == 2 ? 2 : 1, 2, 2, 3>;
+template <typename T> using Low = Grouped<T, 4, 2, 2, 2>;
+template <typename T> using Square = Grouped<T, 4, 4, 2, 2>;
+template <typename T> using Large = Grouped<T, 8, 4, 2, 4>;
+template <typename T> using PairSmall = Grouped<T, 2, 1, 2, 2, 3, 16, true>;
+template <typename T> using PairLow = Grouped<T, 4, 1, 2, 2, 2, 16, true>;
+template <typename T> using Any = Grouped<T, 2, sizeof(T) == 2 ? 2 : 1, 2, 2, 3, 4>;       // (rows on 4-byte boundaries)
+inline bool in_pairs(int slots, int experts) { return (size_t)slots <= PAIR_TOKENS * experts; }
+// No product of these tokens needs more threads than 31 bits count (Small and PairSmall have the most workgroups, Large the most threads).
+template <typename T> static bool one_launch(const ExpertsParams &P) {
+    auto in = [](long long most, int threads) { return most <= INT_MAX / threads; };
+    if (!in(workgroups<true, Small<T>>(P), Small<T>::THREADS) || !in(workgroups<false, Small<T>>(P), Small<T>::THREADS)) return false;
+    if constexpr (sizeof(T) == 2)
+        return in(workgroups<true, Large<T>>(P), Large<T>::THREADS) && in(workgroups<false, Large<T>>(P), Large<T>::THREADS) &&
+               (!in_pairs(P.n * P.k, P.experts) || in(workgroups<false, PairSmall<T>>(P), PairSmall<T>::THREADS));
+    return true;
 }
 // What tiles of S are expected to take (bfloat16), in us.  A CU runs its workgroups in rounds of S::PER_CU; a stage of a round takes what bounds it: bringing
 // it to LDS (50 KB/us and CU), multiplying it (`tflops` a CU), reading the matrices' part (6.2 TB/s), or the way from
@@ -116,18 +152,14 @@ template <bool FIRST, typename S> static double grouped_us(const ExpertsParams &
 // 32 bits: 64 x 32 in three stages, bound by the matrix rate; 64 x 64 and 128 x 128 beside it: 77 tokens to 4 of 16 of 760 x 500 21 / 11, 22 / 15, 55 / 38; of the
 // first experts 256 tokens 166 / 87, 208 / 110, 385 / 198, 1024 tokens 507 / 260, 496 / 259, 596 / 319.
 template <typename T, bool FIRST> static hipError_t grouped_product(const ExpertsParams &P, hipStream_t st) {
-    using Small = Grouped<T, 2, sizeof(T) == 2 ? 2 : 1, 2, 2, 3>;
     if constexpr (sizeof(T) == 2) {
-        using Low = Grouped<T, 4, 2, 2, 2>;
-        using Square = Grouped<T, 4, 4, 2, 2>;
-        using Large = Grouped<T, 8, 4, 2, 4>;
-        const double small = grouped_us<FIRST, Small>(P, 5.4, 2.9), low = grouped_us<FIRST, Low>(P, 5.4, 2.9), square = grouped_us<FIRST, Square>(P, 5.4, 2.9), large = grouped_us<FIRST, Large>(P, 3.3, 8.1);
+        const double small = grouped_us<FIRST, Small<T>>(P, 5.4, 2.9), low = grouped_us<FIRST, Low<T>>(P, 5.4, 2.9), square = grouped_us<FIRST, Square<T>>(P, 5.4, 2.9), large = grouped_us<FIRST, Large<T>>(P, 3.3, 8.1);
         const double least = std::min(std::min(small, low), std::min(square, large));
-        if (large == least) return grouped<T, FIRST, Large>(P, st);
-        if (square == least) return grouped<T, FIRST, Square>(P, st);
-        if (low == least) return grouped<T, FIRST, Low>(P, st);
+        if (large == least) return grouped<T, FIRST, Large<T>>(P, st);
+        if (square == least) return grouped<T, FIRST, Square<T>>(P, st);
+        if (low == least) return grouped<T, FIRST, Low<T>>(P, st);
     }
-    return grouped<T, FIRST, Small>(P, st);
+    return grouped<T, FIRST, Small<T>>(P, st);
 }
 template <typename T> static hipError_t experts(ExpertsParams P, bool &summed, hipStream_t st) {
     P.h_rest = nullptr;
@@ -144,22 +176,19 @@ template <typename T> static hipError_t experts(ExpertsParams P, bool &summed, h
     }
     if ((rc = start(plan_kernel, dim3(P.experts), dim3(1024), 0, st, P.ids, slots, P.experts, P.offs, P.order)) != hipSuccess) return rc;
     if (vec) {
-        const bool pair = sizeof(T) == 2 && (size_t)slots <= PAIR_TOKENS * P.experts;
+        const bool pair = sizeof(T) == 2 && in_pairs(slots, P.experts);
         if (pair) P.h_rest = reinterpret_cast<T *>(P.h) + (size_t)slots * P.ff;
         if ((rc = grouped_product<T, true>(P, st)) != hipSuccess) return rc;
         if constexpr (sizeof(T) == 2) if (pair) {
-            using Small = Grouped<T, 2, 1, 2, 2, 3, 16, true>;
-            using Low = Grouped<T, 4, 1, 2, 2, 2, 16, true>;
-            return grouped_us<false, Low>(P, 5.4, 2.9) < grouped_us<false, Small>(P, 5.4, 2.9) ? grouped<T, false, Low>(P, st) : grouped<T, false, Small>(P, st);
+            return grouped_us<false, PairLow<T>>(P, 5.4, 2.9) < grouped_us<false, PairSmall<T>>(P, 5.4, 2.9) ? grouped<T, false, PairLow<T>>(P, st) : grouped<T, false, PairSmall<T>>(P, st);
         }
         return grouped_product<T, false>(P, st);
     }
     // us a pass with rows on 16-byte boundaries, on 4-byte and on 2-byte ones: 333 tokens to 2 of 8 of 768 x 2048 32, 41, 499; 64 to 6 of 64 of 1536 x 1024
     // 119, 125, 958; 2047 to 8 of 64 of 1536 x 768 251, 364, 7743
     if (rows_on(4)) {
-        using Any = Grouped<T, 2, sizeof(T) == 2 ? 2 : 1, 2, 2, 3, 4>;
-        if ((rc = grouped<T, true, Any>(P, st)) != hipSuccess) return rc;
-        return grouped<T, false, Any>(P, st);
+        if ((rc = grouped<T, true, Any<T>>(P, st)) != hipSuccess) return rc;
+        return grouped<T, false, Any<T>>(P, st);
     }
     if constexpr (sizeof(T) == 2) {
         const int hit = std::min(P.experts, slots), tiles = std::min(hit + (slots - hit) / 16, 65535);
@@ -181,18 +210,50 @@ template <typename T> static hipError_t close(const CloseParams &P, hipStream_t 
     if (P.dim <= 4096) return start(close_rows_kernel<T, 1, 16>, grid, block, 0, st, P);
     return start(close_kernel<T>, grid, block, 0, st, P);
 }
-hipError_t launch_close(const CloseParams &P, int dtype, hipStream_t st) { return dtype == NL_DTYPE_F32 ? close<float>(P, st) : close<bf16>(P, st); }
-hipError_t launch_experts(ExpertsParams P, CloseParams C, int dtype, hipStream_t st) {
+// the rows from token t on, n of them
+static CloseParams rows_from(CloseParams P, long long t, int n, size_t size) {
+    P.x = behind(P.x, t * P.ldx); P.add = behind(P.add, t * P.ldadd); P.base = behind(P.base, t * P.ldbase); P.d = behind(P.d, t * P.ldd, size);
+    P.part = behind(P.part, t * P.k * P.dim); P.ids = behind(P.ids, t * P.k); P.gate = behind(P.gate, t * P.ldgate);
+    P.x_out = behind(P.x_out, t * P.ldxo); P.h = behind(P.h, t * P.ldh, size); P.y = behind(P.y, t * P.ldy, size);
+    P.n = n;
+    return P;
+}
+hipError_t launch_close(const CloseParams &P, int dtype, hipStream_t st) {
+    hipError_t rc = hipSuccess;
+    for (long long t = 0; t < P.n && rc == hipSuccess; t += CLOSE_TOKENS) {
+        const CloseParams Q = rows_from(P, t, (int)std::min<long long>(P.n - t, CLOSE_TOKENS), dtype == NL_DTYPE_F32 ? 4 : 2);
+        rc = dtype == NL_DTYPE_F32 ? close<float>(Q, st) : close<bf16>(Q, st);
+    }
+    return rc;
+}
+template <typename T> static hipError_t experts_and_close(ExpertsParams P, CloseParams C, hipStream_t st) {
     C.part = P.part; C.ids = P.ids; C.k = P.k; C.experts = P.experts; C.n = P.n; C.dim = P.dim;
     P.y = C.x_out ? nullptr : C.y;
     P.ldy = C.ldy;
     P.res_out = C.post || C.gate || C.h ? nullptr : C.x_out;       // (nothing that needs the whole row)
     P.ldo = C.ldxo; P.res = C.x; P.ldres = C.ldx; P.add = C.add; P.ldadd = C.ldadd; P.scale = C.scale;
     bool summed = false;
-    const hipError_t rc = dtype == NL_DTYPE_F32 ? experts<float>(P, summed, st) : experts<bf16>(P, summed, st);
+    const hipError_t rc = experts<T>(P, summed, st);
     if (rc != hipSuccess || (summed && (P.y || P.res_out))) return rc;
     if (summed) { C.ids = nullptr; C.k = 1; }
-    return launch_close(C, dtype, st);
+    return close<T>(C, st);
+}
+template <typename T> static hipError_t experts_in_parts(const ExpertsParams &P, const CloseParams &C, hipStream_t st) {
+    // as many tokens as a launch counts; behind one another the parts share the workspace
+    ExpertsParams Q = P;
+    Q.n = std::min(P.n, CLOSE_TOKENS);
+    while (Q.n > 1 && !one_launch<T>(Q)) Q.n = (Q.n + 1) / 2;
+    const int most = Q.n;
+    hipError_t rc = hipSuccess;
+    for (long long t = 0; t < P.n && rc == hipSuccess; t += most) {
+        Q.n = (int)std::min<long long>(P.n - t, most);
+        Q.x = behind(P.x, t * P.ldx, sizeof(T)); Q.ids = behind(P.ids, t * P.k); Q.weights = behind(P.weights, t * P.k);
+        rc = experts_and_close<T>(Q, rows_from(C, t, Q.n, sizeof(T)), st);
+    }
+    return rc;
+}
+hipError_t launch_experts(const ExpertsParams &P, const CloseParams &C, int dtype, hipStream_t st) {
+    return dtype == NL_DTYPE_F32 ? experts_in_parts<float>(P, C, st) : experts_in_parts<bf16>(P, C, st);
 }
 
 }  // namespace nl
