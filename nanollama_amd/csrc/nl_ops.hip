@@ -272,6 +272,8 @@ int fail(int code, const char *fmt, ...) {
     return code;
 }
 
+int off_elements(const char *name) { return fail(NL_ERR_INVALID, "%s: an array is not on a boundary of its elements", name); }
+
 // the caller's current device, given back at the end
 struct OnDevice {
     int before = -1;
@@ -327,6 +329,7 @@ int nl_op_route(int device, void *stream, const nl_route_desc *d, int n, const f
     if (!(d->scale - d->scale == 0.f)) return fail(NL_ERR_INVALID, "route: scale is not finite");
     if (n == 0) return NL_OK;
     if (!logits || !ids || !weights) return fail(NL_ERR_INVALID, "route: null argument");
+    if (!on(logits, 4) || !on(bias, 4) || !on(ids, 4) || !on(weights, 4)) return off_elements("route");
     if (ld < d->experts) return fail(NL_ERR_INVALID, "route: ld %lld is less than %d experts", (long long)ld, d->experts);
     RouteParams P{};
     P.logits = logits; P.bias = bias; P.ld = ld; P.n = n; P.experts = d->experts; P.k = d->per_token; P.sigmoid = d->score == NL_SCORE_SIGMOID;
@@ -346,7 +349,7 @@ int nl_op_experts(int device, void *stream, const nl_experts_desc *d, int n, con
     if (!x || !ids || !weights || !gate || !up || !down || !y || !workspace) return fail(NL_ERR_INVALID, "experts: null argument");
     if (ldx < d->dim || ldy < d->dim) return fail(NL_ERR_INVALID, "experts: ldx %lld and ldy %lld, rows have %d elements", (long long)ldx, (long long)ldy, d->dim);
     const size_t size = d->dtype == NL_DTYPE_F32 ? 4 : 2;
-    if (!on(x, size) || !on(gate, size) || !on(up, size) || !on(down, size) || !on(y, size)) return fail(NL_ERR_INVALID, "experts: an array is not on a boundary of its elements");
+    if (!on(x, size) || !on(gate, size) || !on(up, size) || !on(down, size) || !on(y, size) || !on(ids, 4) || !on(weights, 4)) return off_elements("experts");
     const ExpertsLayout L = experts_layout(n, d->per_token, d->experts, d->dim, d->ff, d->dtype);
     if (workspace_bytes < L.bytes) return fail(NL_ERR_INVALID, "experts: workspace of %llu bytes, %llu are needed", (unsigned long long)workspace_bytes, (unsigned long long)L.bytes);
     if (!on(workspace, 16)) return fail(NL_ERR_INVALID, "experts: workspace is not on a 16-byte boundary");
@@ -369,6 +372,8 @@ int nl_op_residual_norm(int device, void *stream, const nl_residual_norm_desc *d
     if (!x || !b || !x_out || (h && !pre)) return fail(NL_ERR_INVALID, "residual_norm: null argument");
     if (ldx < d->dim || ldb < d->dim || ldxo < d->dim || (gate && ldgate != 0 && ldgate < d->dim) || (h && ldh < d->dim))
         return fail(NL_ERR_INVALID, "residual_norm: a row distance is less than %d", d->dim);
+    const size_t size = d->dtype == NL_DTYPE_F32 ? 4 : 2;
+    if (!on(x, 4) || !on(b, size) || !on(post, 4) || !on(gate, 4) || (h && !on(pre, 4)) || !on(x_out, 4) || !on(h, size)) return off_elements("residual_norm");
     if (x_out == x && ldxo != ldx) return fail(NL_ERR_INVALID, "residual_norm: x_out is x with other rows");
     CloseParams P{};
     P.x = x; P.ldx = ldx; P.d = b; P.ldd = ldb; P.post = post; P.gate = gate; P.ldgate = ldgate; P.pre = pre; P.x_out = x_out; P.ldxo = ldxo; P.h = h; P.ldh = ldh;
