@@ -80,6 +80,7 @@ NL_API int nl_op_residual_norm(int device, void *stream, const nl_residual_norm_
  *     layers.N.ff.router                       [experts, dim],  ff.router_bias [experts] with bias (sigmoid scores only, joins the choice alone)
  *     layers.N.ff.experts.gate / up            [experts * ff, dim], expert behind expert
  *     layers.N.ff.experts.down                 [experts * dim, ff]
+ * A call that fails, for want of memory too, leaves the handle as it was.
  * In bfloat16 a token's choice can differ between decode and prompt launches where two keys lie within the rounding of the router's operand. */
 typedef struct {
     int32_t experts, per_token, ff, act;        /* ff: width of an expert; act: NL_ACT_* */

@@ -1019,9 +1019,20 @@ int nl_stack_experts(nl_handle e, int layer, const nl_stack_experts_desc *d) {
     HIPCK(e, hipSetDevice(e->c.device));
     const size_t one = (size_t)d->experts * d->ff * e->c.dim * e->esize();
     size_t &bw = e->bytes_weights;
+    const size_t held = bw, allocs = e->allocs.size();
     int rc;
     if ((rc = mat_alloc(e, L.router, d->experts, e->c.dim)) || (rc = dev_alloc(e, L.norm2, (size_t)e->c.dim * 4, bw)) || (rc = dev_alloc(e, L.xgate, one, bw)) ||
-        (rc = dev_alloc(e, L.xup, one, bw)) || (rc = dev_alloc(e, L.xdown, one, bw)) || (d->bias && (rc = dev_alloc(e, L.routerb, (size_t)d->experts * 4, bw)))) return rc;
+        (rc = dev_alloc(e, L.xup, one, bw)) || (rc = dev_alloc(e, L.xdown, one, bw)) || (d->bias && (rc = dev_alloc(e, L.routerb, (size_t)d->experts * 4, bw)))) {
+        // as before the call: it may come again with a smaller description
+        (void)hipStreamSynchronize(e->stream);
+        for (; e->allocs.size() > allocs; e->allocs.pop_back()) (void)hipFree(e->allocs.back());
+        (void)hipGetLastError();                         // (the next launch's check asks for it)
+        bw = held;
+        L.router = Mat{};
+        L.norm2 = L.routerb = nullptr;
+        L.xgate = L.xup = L.xdown = nullptr;
+        return rc;
+    }
     L.x = *d;
     return NL_OK;
 }
