@@ -272,6 +272,11 @@ int fail(int code, const char *fmt, ...) {
     return code;
 }
 
+// an error of the runtime's is told here and not kept for the program's next look at it
+int hip_error(const char *name, hipError_t rc) {
+    (void)hipGetLastError();
+    return fail(NL_ERR_HIP, "%s: %s", name, hipGetErrorString(rc));
+}
 int off_elements(const char *name) { return fail(NL_ERR_INVALID, "%s: an array is not on a boundary of its elements", name); }
 
 // the caller's current device, given back at the end
@@ -291,17 +296,20 @@ template <typename F> int on_device(const char *name, int device, void *stream, 
     static std::atomic<int> seen{0};                     // devices, once there are any
     int ndev = seen.load(std::memory_order_relaxed);
     if (ndev == 0) {
-        if (hipGetDeviceCount(&ndev) != hipSuccess || ndev == 0) return fail(NL_ERR_HIP, "%s: no HIP device", name);
+        if (hipGetDeviceCount(&ndev) != hipSuccess || ndev == 0) {
+            (void)hipGetLastError();
+            return fail(NL_ERR_HIP, "%s: no HIP device", name);
+        }
         seen.store(ndev, std::memory_order_relaxed);
     }
     if (device < 0 || device >= ndev) return fail(NL_ERR_INVALID, "%s: device %d of %d", name, device, ndev);
     OnDevice on(device);
-    if (on.rc != hipSuccess) return fail(NL_ERR_HIP, "%s: %s", name, hipGetErrorString(on.rc));
+    if (on.rc != hipSuccess) return hip_error(name, on.rc);
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     hipDevice_t at = device;
     if (st && hipStreamGetDevice(st, &at) == hipSuccess && at != device) return fail(NL_ERR_INVALID, "%s: the stream is of device %d, not %d", name, at, device);
     const hipError_t rc = launches(st);
-    return rc == hipSuccess ? (int)NL_OK : fail(NL_ERR_HIP, "%s: %s", name, hipGetErrorString(rc));
+    return rc == hipSuccess ? (int)NL_OK : hip_error(name, rc);
 }
 
 const char *experts_error(const nl_experts_desc *d, int n) {
