@@ -55,7 +55,7 @@ def _check(rc: int) -> None:
 
 @lru_cache(maxsize=256)
 def _desc(kind, *fields):
-    """A description; the library only reads it."""
+    """A description by its values (plain numbers: anything else would be found again by its identity); the library only reads it."""
     return kind(*fields)
 
 
@@ -72,7 +72,7 @@ def route(logits, ids, weights, score: str = "softmax", bias=None, renorm: bool 
     ip, _ = _array("ids", ids, "int32", (n, k), dev)
     wp, _ = _array("weights", weights, "float32", (n, k), dev)
     bp = None if bias is None else _array("bias", bias, "float32", (count,), dev)[0]
-    d = _desc(_lib.NlRouteDesc, count, k, _one_of("score", score, SCORES), int(renorm), scale)
+    d = _desc(_lib.NlRouteDesc, count, k, _one_of("score", score, SCORES), int(renorm), float(scale))
     _check(_lib.stack_lib().nl_op_route(dev, stream, d, n, lp, ld, bp, ip, wp))
 
 
@@ -116,5 +116,5 @@ def residual_norm(x, d, x_out, h=None, pre=None, post=None, gate=None, scale: fl
     gp, ldg = None, 0
     if gate is not None:
         gp, ldg = (vec("gate", gate), 0) if len(gate.shape) == 1 else _array("gate", gate, "float32", (n, dim), dev, strided=True)
-    desc = _desc(_lib.NlResidualNormDesc, dim, _one_of("type of d", t, DTYPES), eps, scale)
+    desc = _desc(_lib.NlResidualNormDesc, dim, _one_of("type of d", t, DTYPES), float(eps), float(scale))
     _check(_lib.stack_lib().nl_op_residual_norm(dev, stream, desc, n, xp, ldx, dp, ldd, vec("post", post), gp, ldg, vec("pre", pre), op, ldo, hp, ldh))
