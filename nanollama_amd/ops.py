@@ -53,10 +53,17 @@ def _check(rc: int) -> None:
         raise _lib.NlError(rc, (_lib.stack_lib().nl_last_error(None) or b"").decode())
 
 
+def _int32(n: int) -> int:
+    """A number that the library takes in 32 bits (ctypes would cut it off without a word)."""
+    if not -1 << 31 <= n < 1 << 31:
+        raise ValueError(f"{n}: more than 32 bits hold")
+    return n
+
+
 @lru_cache(maxsize=256)
 def _desc(kind, *fields):
     """A description by its values (plain numbers: anything else would be found again by its identity); the library only reads it."""
-    return kind(*fields)
+    return kind(*(f if isinstance(f, float) else _int32(f) for f in fields))
 
 
 def _one_of(name: str, value: str, table) -> int:
@@ -73,13 +80,13 @@ def route(logits, ids, weights, score: str = "softmax", bias=None, renorm: bool 
     wp, _ = _array("weights", weights, "float32", (n, k), dev)
     bp = None if bias is None else _array("bias", bias, "float32", (count,), dev)[0]
     d = _desc(_lib.NlRouteDesc, count, k, _one_of("score", score, SCORES), int(renorm), float(scale))
-    _check(_lib.stack_lib().nl_op_route(dev, stream, d, n, lp, ld, bp, ip, wp))
+    _check(_lib.stack_lib().nl_op_route(dev, stream, d, _int32(n), lp, ld, bp, ip, wp))
 
 
 def experts_workspace(n: int, per_token: int, count: int, dim: int, ff: int, dtype: str = "bfloat16") -> int:
     """Bytes that experts() needs beside its arrays for up to n tokens."""
     d = _desc(_lib.NlExpertsDesc, count, per_token, dim, ff, 0, _one_of("dtype", dtype, DTYPES))
-    size = _lib.stack_lib().nl_op_experts_workspace(d, n)
+    size = _lib.stack_lib().nl_op_experts_workspace(d, _int32(n))
     if size == 0:
         _check(-1)
     return size
@@ -99,7 +106,7 @@ def experts(x, ids, weights, gate, up, down, out, workspace, act: str = "silu", 
     size = workspace.numel()
     sp, _ = _array("workspace", workspace, "uint8", (size,), dev)
     d = _desc(_lib.NlExpertsDesc, count, k, dim, ff, _one_of("act", act, ACTIVATIONS), _one_of("type of x", t, DTYPES))
-    _check(_lib.stack_lib().nl_op_experts(dev, stream, d, n, xp, ldx, ip, wp, gp, up_, dp, yp, ldy, sp, size))
+    _check(_lib.stack_lib().nl_op_experts(dev, stream, d, _int32(n), xp, ldx, ip, wp, gp, up_, dp, yp, ldy, sp, size))
 
 
 def residual_norm(x, d, x_out, h=None, pre=None, post=None, gate=None, scale: float = 1.0, eps: float = 1e-5, stream: int = 0) -> None:
@@ -117,4 +124,4 @@ def residual_norm(x, d, x_out, h=None, pre=None, post=None, gate=None, scale: fl
     if gate is not None:
         gp, ldg = (vec("gate", gate), 0) if len(gate.shape) == 1 else _array("gate", gate, "float32", (n, dim), dev, strided=True)
     desc = _desc(_lib.NlResidualNormDesc, dim, _one_of("type of d", t, DTYPES), float(eps), float(scale))
-    _check(_lib.stack_lib().nl_op_residual_norm(dev, stream, desc, n, xp, ldx, dp, ldd, vec("post", post), gp, ldg, vec("pre", pre), op, ldo, hp, ldh))
+    _check(_lib.stack_lib().nl_op_residual_norm(dev, stream, desc, _int32(n), xp, ldx, dp, ldd, vec("post", post), gp, ldg, vec("pre", pre), op, ldo, hp, ldh))

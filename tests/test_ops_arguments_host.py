@@ -1,4 +1,6 @@
 """Arguments of nanollama_amd.ops on their way into the library, without a GPU."""
+import math
+
 import pytest
 
 from nanollama_amd import _lib, ops
@@ -44,3 +46,25 @@ def test_numbers_are_read_at_every_call(library):
         ops.residual_norm(f32(4, 8), f32(4, 8), f32(4, 8), scale=scale, eps=eps)
         (_, route, _), (_, close, _) = library.seen[-2:]
         assert route["scale"] == s and close["scale"] == s and close["eps"] == e
+
+
+def far(*shape, dtype="float32"):
+    a = Fake(1, dtype=dtype)
+    a.shape = shape
+    a._stride = tuple(math.prod(shape[i + 1:]) for i in range(len(shape)))
+    return a
+
+
+@pytest.mark.parametrize("n", [1 << 31, (1 << 32) + 4])
+def test_numbers_that_32_bits_do_not_hold_are_refused(library, n):
+    ids, w = far(n, 1, dtype="int32"), far(n, 1)
+    calls = [lambda: ops.route(far(n, 8), ids, w), lambda: ops.residual_norm(far(n, 8), far(n, 8), far(n, 8)),
+             lambda: ops.experts(far(n, 8), ids, w, far(4, 8, 8), far(4, 8, 8), far(4, 8, 8), far(n, 8), Fake(100, dtype="uint8")),
+             lambda: ops.experts_workspace(n, 1, 4, 8, 8), lambda: ops.experts_workspace(4, n, 4, 8, 8), lambda: ops.experts_workspace(4, 1, 4, n, 8),
+             lambda: ops.residual_norm(far(1, n), far(1, n), far(1, n)), lambda: ops.route(far(1, n), far(1, 2, dtype="int32"), far(1, 2))]
+    for call in calls:
+        with pytest.raises(ValueError, match=f"{n}: more than 32 bits hold"):
+            call()
+    assert not library.seen
+    ops.residual_norm(far((1 << 31) - 1, 1), far((1 << 31) - 1, 1), far((1 << 31) - 1, 1))
+    assert library.seen[0][2] == (1 << 31) - 1
