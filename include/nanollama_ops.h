@@ -8,10 +8,11 @@
  * Layer-stack models call the same kernels for layers that nl_stack_experts (below) has given experts.
  *
  * Conventions.  Pointers are device memory of `device` that the caller owns, unless a comment says otherwise; nothing is kept behind a
- * return, and no call allocates, synchronises or copies to the host: work is queued on `stream` (a hipStream_t of `device`, NULL: its
- * default stream), and a call may be captured into a graph.  The caller's current device is as it was behind every call.  Arrays are
- * row-major and on a boundary of their elements; ld* are elements from a row to the next.  n == 0 queues nothing.  Calls on different
- * threads and streams do not disturb each other as long as their outputs and workspaces do not overlap.  0 or a negative nl_status; nl_last_error(NULL) has this thread's message.
+ * return, and no call allocates, synchronises or copies to the host: work is queued on `stream` (a hipStream_t of `device`; NULL,
+ * hipStreamLegacy, hipStreamPerThread: its default streams), and a call may be captured into a graph.  The caller's current device is as
+ * it was behind every call.  Arrays are row-major and on a boundary of their elements; ld* are elements from a row to the next.  n == 0
+ * queues nothing.  Calls on different threads and streams do not disturb each other as long as their outputs and workspaces do not
+ * overlap.  0 or a negative nl_status; nl_last_error(NULL) has this thread's message.
  * Element type `dtype`: NL_DTYPE_BF16 or NL_DTYPE_F32 (nanollama_stack.h); sums, scores, weights and norms are 32-bit either way.
  */
 #ifndef NANOLLAMA_OPS_H

@@ -305,9 +305,16 @@ template <typename F> int on_device(const char *name, int device, void *stream, 
     if (device < 0 || device >= ndev) return fail(NL_ERR_INVALID, "%s: device %d of %d", name, device, ndev);
     OnDevice on(device);
     if (on.rc != hipSuccess) return hip_error(name, on.rc);
-    const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    // the default streams' handles are no streams: they are of the device that is current, and a runtime that does not know hipStreamLegacy yet ends the
+    // process when it is asked for that one's
+    if (st == hipStreamLegacy) st = nullptr;
     hipDevice_t at = device;
-    if (st && hipStreamGetDevice(st, &at) == hipSuccess && at != device) return fail(NL_ERR_INVALID, "%s: the stream is of device %d, not %d", name, at, device);
+    if (st && st != hipStreamPerThread) {
+        const hipError_t rc = hipStreamGetDevice(st, &at);
+        if (rc != hipSuccess) return hip_error(name, rc);
+    }
+    if (at != device) return fail(NL_ERR_INVALID, "%s: the stream is of device %d, not %d", name, at, device);
     const hipError_t rc = launches(st);
     return rc == hipSuccess ? (int)NL_OK : hip_error(name, rc);
 }

@@ -27,3 +27,14 @@ def test_an_error_is_not_the_next_calls():
     ops.route(l, ids, w)
     sync()
     assert np.array_equal(ids.numpy(), np.tile([[7, 6]], (4, 1)))
+
+
+@pytest.mark.parametrize("stream", [0, 1, 2])             # the default stream, by its other name, and this thread's own
+def test_default_streams_have_handles(stream):
+    rng = np.random.default_rng(stream)
+    logits = rng.standard_normal((5, 8)).astype(np.float32)
+    l, ids, w = DeviceArray(logits), DeviceArray(np.zeros((5, 2), np.int32)), DeviceArray(np.zeros((5, 2), np.float32))
+    sync()
+    ops.route(l, ids, w, stream=stream)
+    sync()
+    assert np.array_equal(ids.numpy(), np.argsort(-logits, axis=1, kind="stable")[:, :2])
