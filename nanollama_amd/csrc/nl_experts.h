@@ -30,14 +30,16 @@ __device__ __forceinline__ unsigned order_u32(float v) {
 __device__ __forceinline__ float order_f32(unsigned u) { return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u); }
 
 // A wavefront per token; expert e is element e / 64 of lane e % 64.
-// With a bias the keys sigmoid(l) + b are 32-bit numbers within KEY_ERR (1 + |b|) of the exact ones: where two neighbours among the chosen ones and
-// the best one left are nearer than twice that, the keys that matter are computed again in 64 bits.
+// With a bias the keys sigmoid(l) + b are 32-bit numbers within key_err(b) of the exact ones: where two neighbours among the chosen ones, or the last of them and
+// anyone left, are not apart by what both may be off, the keys that matter are computed again in 64 bits.  Every expert counts with its own error: a few that
+// a large negative bias keeps out do not make the others near (8191 tokens to 8 of 256 with four biases of -1e9: 11 us; 29 with the largest error for all).
 // Bound by its instructions, about 500 vector ones a token: 8191 tokens to 8 of 256 12.8 us (reading the logits alone 2); 18 where the second look, which one
 // token in 200 needs, went over all experts; 19 where the largest was looked for k times instead of the border once.  One token 2.5 us, 64 to 6 of 96 4.5.
-constexpr float KEY_ERR = 1e-6f;
+// sigmoid_f32 is within 3e-7, the sum within half a step; past 2^24, where a sigmoid is lost in the sum, within 1 (a number that rounds to itself there)
+__device__ __forceinline__ float key_err(float b) { return fminf(1e-6f * (1.f + fabsf(b)), 2.f); }
 template <int NE>
 __global__ void __launch_bounds__(256) route_kernel(RouteParams P) {
-    __shared__ __align__(16) f32x4 chosen[4][64];      // of a token: key, number, logit
+    __shared__ __align__(16) f32x4 chosen[4][64];      // of a token: key, number, logit, bias
     const int wave = threadIdx.x >> 6, t = blockIdx.x * 4 + wave, lane = threadIdx.x & 63;
     if (t >= P.n) return;
     const float *row = P.logits + (long long)t * P.ld;
@@ -58,12 +60,10 @@ __global__ void __launch_bounds__(256) route_kernel(RouteParams P) {
     }
     m = order_f32(wave_umax(order_u32(m)));
     unsigned key[NE];
-    float off = 0.f;                                     // how far keys may be off, together
 #pragma unroll
     for (int i = 0; i < NE; i++) {
         const float v = P.bias ? sigmoid_f32(l[i]) + b[i] : l[i];
         key[i] = out[i] ? 0 : order_u32(v);
-        if (P.bias && !out[i]) off = fmaxf(off, 2.f * KEY_ERR * (1.f + fminf(fabsf(b[i]), 1e30f)));
     }
     int pick = -1;                                       // lane j: the j-th choice
     float score = 0.f;                                   // ... its logit
@@ -99,11 +99,11 @@ __global__ void __launch_bounds__(256) route_kernel(RouteParams P) {
         }
         // one behind the other by number, then by rank
         int at = 0;
-        unsigned left = 0;
+        float left = -INFINITY;                          // (with a bias) the most that a key left may be
 #pragma unroll
         for (int i = 0; i < NE; i++) {
-            if (in[i] >> lane & 1) chosen[wave][at + __popcll(in[i] & ((1ull << lane) - 1))] = f32x4{__uint_as_float(key[i]), __int_as_float(lane + 64 * i), l[i], 0.f};
-            else left = max(left, key[i]);
+            if (in[i] >> lane & 1) chosen[wave][at + __popcll(in[i] & ((1ull << lane) - 1))] = f32x4{__uint_as_float(key[i]), __int_as_float(lane + 64 * i), l[i], b[i]};
+            else if (P.bias && key[i]) left = fmaxf(left, order_f32(key[i]) + key_err(b[i]));
             at += __popcll(in[i]);
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");         // (one wavefront's: no barrier)
@@ -121,25 +121,24 @@ __global__ void __launch_bounds__(256) route_kernel(RouteParams P) {
         if (lane < want) { pick = __float_as_int(sorted[1]); score = sorted[2]; }
         bool near = false;
         float last = 0.f;
-        if (P.bias) {                                    // a neighbour, or the best that is left, too near to be sure
-            last = __uint_as_float(wave_umax(__float_as_uint(off)));
-            const float far = last, v = order_f32(__float_as_uint(sorted[0])), next = __shfl_down(v, 1);
-            left = wave_umax(left);
-            if (lane + 1 < want) near = !(v - next > far);
-            if (lane + 1 == want && left) near = !(v - order_f32(left) > far);
+        if (P.bias) {
+            const float v = order_f32(__float_as_uint(sorted[0])), err = key_err(sorted[3]), next = __shfl_down(v + err, 1);
+            left = order_f32(wave_umax(order_u32(left)));
+            if (lane < want) near = !(v - err > (lane + 1 < want ? next : left));
+            if (lane + 1 == want && left == -INFINITY) near = false;
             near = __ballot(near) != 0;
-            last = lane_value(v, max(want - 1, 0)) - 2.f * far;        // nothing below can be among the chosen ones
+            last = order_f32(~wave_umax(lane < want ? ~order_u32(v - err) : 0u));     // nothing that cannot reach it can be among the chosen ones
         }
         int few = 0;                                     // that many can
         if (near) {
 #pragma unroll
-            for (int i = 0; i < NE; i++) few += __popcll(__ballot(key[i] && order_f32(key[i]) >= last));
+            for (int i = 0; i < NE; i++) few += __popcll(__ballot(key[i] && order_f32(key[i]) + key_err(b[i]) >= last));
         }
         if (near && few <= 64) {                         // a key in 64 bits a lane, then by rank
             int to = 0;
 #pragma unroll
             for (int i = 0; i < NE; i++) {
-                const bool can = key[i] && order_f32(key[i]) >= last;
+                const bool can = key[i] && order_f32(key[i]) + key_err(b[i]) >= last;
                 const unsigned long long cans = __ballot(can);
                 if (can) chosen[wave][to + __popcll(cans & ((1ull << lane) - 1))] = f32x4{l[i], b[i], __int_as_float(lane + 64 * i), 0.f};
                 to += __popcll(cans);
