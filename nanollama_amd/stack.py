@@ -191,6 +191,20 @@ def _layer_desc(layer: StackLayer) -> _lib.NlLayerDesc:
     return d
 
 
+def rows_and_columns(spec: StackSpec, name: str, source: str, shape: Tuple[int, ...]) -> Tuple[int, int]:
+    """A tensor of the file as nl_upload_tensor takes it: a vector is a row, experts' matrices [experts, rows, columns] lie expert behind expert."""
+    if len(shape) == 1:
+        return 1, shape[0]
+    if len(shape) == 3 and ".ff.experts." in name:
+        x = spec.layers[int(name.split(".")[1])].experts
+        if shape[0] != x.experts:
+            raise ValueError(f"tensor {source}: {list(shape)}, expected {x.experts} experts")
+        return shape[0] * shape[1], shape[2]
+    if len(shape) != 2:
+        raise ValueError(f"tensor {source}: {len(shape)} dimensions")
+    return shape[0], shape[1]
+
+
 def load_stack_model(spec: StackSpec, get: Callable[[str], Tuple[str, np.ndarray]], device: int = 0, max_streams: int = 1,
                      seq_len: int = 0, dtype: str = "bfloat16", max_step_tokens: int = 0, flags: int = 0, verbose: bool = False) -> StackModel:
     """get(name in the weight file) -> (dtype tag, array), as SafetensorsFile.get."""
@@ -218,7 +232,7 @@ def load_stack_model(spec: StackSpec, get: Callable[[str], Tuple[str, np.ndarray
             if tag not in ("F32", "BF16"):
                 raise ValueError(f"tensor {source}: type {tag} (float32 and bfloat16 are taken)")
             x = np.ascontiguousarray(x)
-            rows, cols = (1, x.shape[0]) if x.ndim == 1 else (x.size // x.shape[-1], x.shape[-1])      # (experts' matrices: expert behind expert)
+            rows, cols = rows_and_columns(spec, name, source, x.shape)
             params += x.size
             _lib.check(h, L.nl_upload_tensor(h, name.encode(), 0 if tag == "F32" else 30, x.ctypes.data, x.nbytes, rows, cols), L)
         _lib.check(h, L.nl_finalize(h), L)
