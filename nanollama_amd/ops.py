@@ -26,17 +26,19 @@ def _type(a) -> str:
     return t
 
 
-def _shape(name: str, a, dimensions: int):
-    if len(a.shape) != dimensions:
-        raise ValueError(f"{name}: {len(a.shape)} dimensions, expected {dimensions}")
-    return a.shape
+def _shapes(**arrays) -> None:
+    """Refuses arrays that do not have so many dimensions: name=(array, dimensions)."""
+    for name, (a, dimensions) in arrays.items():
+        if len(a.shape) != dimensions:
+            raise ValueError(f"{name}: {len(a.shape)} dimensions, expected {dimensions}")
 
 
 def _device(name: str, a) -> int:
     """Where an operator runs: with its first array."""
-    if a.device.index is None:
+    index = a.device.index
+    if index is None:
         raise ValueError(f"{name}: in host memory")
-    return a.device.index
+    return index
 
 
 def _array(name: str, a, dtype: str, shape: tuple, device=None, strided=False):
@@ -87,7 +89,11 @@ def _one_of(name: str, value: str, table) -> int:
 
 def route(logits, ids, weights, score: str = "softmax", bias=None, renorm: bool = True, scale: float = 1.0, stream: int = 0) -> None:
     """logits [n, experts] float32 -> ids [n, k] int32, weights [n, k] float32; bias [experts] float32 joins sigmoid scores in the choice alone."""
-    (n, count), (_, k), dev = _shape("logits", logits, 2), _shape("ids", ids, 2), _device("logits", logits)
+    try:
+        (n, count), (_, k) = logits.shape, ids.shape
+    except ValueError:
+        _shapes(logits=(logits, 2), ids=(ids, 2))
+    dev = _device("logits", logits)
     lp, ld = _array("logits", logits, "float32", (n, count), strided=True)
     ip, _ = _array("ids", ids, "int32", (n, k), dev)
     wp, _ = _array("weights", weights, "float32", (n, k), dev)
@@ -108,7 +114,11 @@ def experts_workspace(n: int, per_token: int, count: int, dim: int, ff: int, dty
 def experts(x, ids, weights, gate, up, down, out, workspace, act: str = "silu", stream: int = 0) -> None:
     """out [n, dim] = sum over j of weights[:, j] * down[e] (act(gate[e] x) * up[e] x), e = ids[:, j]; an id that is no expert adds nothing.
     x [n, dim], gate and up [experts, ff, dim], down [experts, dim, ff], all of one type; workspace: experts_workspace() bytes of its own."""
-    (n, dim), (count, ff, _), (_, k), dev, t = _shape("x", x, 2), _shape("gate", gate, 3), _shape("ids", ids, 2), _device("x", x), _type(x)
+    try:
+        (n, dim), (count, ff, _), (_, k) = x.shape, gate.shape, ids.shape
+    except ValueError:
+        _shapes(x=(x, 2), gate=(gate, 3), ids=(ids, 2))
+    dev, t = _device("x", x), _type(x)
     xp, ldx = _array("x", x, t, (n, dim), strided=True)
     ip, _ = _array("ids", ids, "int32", (n, k), dev)
     wp, _ = _array("weights", weights, "float32", (n, k), dev)
@@ -125,7 +135,8 @@ def experts(x, ids, weights, gate, up, down, out, workspace, act: str = "silu", 
 def residual_norm(x, d, x_out, h=None, pre=None, post=None, gate=None, scale: float = 1.0, eps: float = 1e-5, stream: int = 0) -> None:
     """x_out = x + scale * gate * (norm(d) * post), or d itself without post; h = norm(x_out) * pre.  x, x_out [n, dim] float32 (x_out may be x),
     d, h [n, dim] of one type, gate [dim] or [n, dim], post, pre [dim] float32."""
-    (n, dim), dev, t = _shape("x", x, 2), _device("x", x), _type(d)
+    _shapes(x=(x, 2))
+    (n, dim), dev, t = x.shape, _device("x", x), _type(d)
     xp, ldx = _array("x", x, "float32", (n, dim), strided=True)
     dp, ldd = _array("d", d, t, (n, dim), dev, strided=True)
     op, ldo = _array("x_out", x_out, "float32", (n, dim), dev, strided=True)
