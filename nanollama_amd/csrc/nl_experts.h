@@ -33,8 +33,9 @@ __device__ __forceinline__ float order_f32(unsigned u) { return __uint_as_float(
 // With a bias the keys sigmoid(l) + b are 32-bit numbers within key_err(b) of the exact ones: where two neighbours among the chosen ones, or the last of them and
 // anyone left, are not apart by what both may be off, the keys that matter are computed again in 64 bits.  Every expert counts with its own error: a few that
 // a large negative bias keeps out do not make the others near (8191 tokens to 8 of 256 with four biases of -1e9: 11 us; 29 with the largest error for all).
-// Bound by its instructions, about 500 vector ones a token: 8191 tokens to 8 of 256 12.8 us (reading the logits alone 2); 18 where the second look, which one
-// token in 200 needs, went over all experts; 19 where the largest was looked for k times instead of the border once.  One token 2.5 us, 64 to 6 of 96 4.5.
+// Bound by its instructions, about 500 vector ones a token: 8191 tokens to 8 of 256 11.5 us (reading the logits alone 2); 18 where the second look, which one
+// token in 200 needs, went over all experts; 19 where the largest was looked for k times instead of the border once.  To 8 of 64, 384, 512 and 1024 7.4, 17,
+// 18 and 47, to 32 of 1024 58 (beyond 256 experts registers leave six wavefronts a SIMD, beyond 512 two).  One token 2.5 us, 64 to 6 of 96 4.5.
 // sigmoid_f32 is within 3e-7, the sum within half a step; past 2^24, where a sigmoid is lost in the sum, within 1 (a number that rounds to itself there)
 __device__ __forceinline__ float key_err(float b) { return fminf(1e-6f * (1.f + fabsf(b)), 2.f); }
 template <int NE>
@@ -485,9 +486,9 @@ __global__ void __launch_bounds__(256) experts_token_second_kernel(ExpertsParams
 // Prompts: WR x WT wavefronts of RTW row tiles x NTW token tiles each; 128 bytes of every row at a time go through a ring of two or three LDS stages by
 // LDS-DMA, a piece of 8 rows (UNIT 16 bytes a lane), whole lines of the rows as they lie, or of 2 (UNIT 4, for rows that start on 4-byte boundaries only).  In
 // LDS the 16-byte run q of row r is at q ^ (r % 8), so that the 16 rows of a fragment are read from all banks.  FIRST: row tiles alternate between gate and up.
-// Bound by what a CU's L1 has on its way: about 64 KB, 1.1 us each.  Two workgroups of 128 x 128 take 1.05 us a stage (43 KB/us of DMA, 1.0 PFLOP/s over the chip); as long
-// where nobody waits for a stage, 5 us less of 128 where LDS is not read, 48 less without the DMA; one of 256 x 256 1.8 us (1.2 PFLOP/s), half the
-// bytes a product, but as few and as large workgroups as leave CUs idle.  Tokens that fill a small part of a tile, and few rounds, cost more than either.
+// Bound by bringing the stages: 2047 tokens to 8 of 64 of 1536 x 768, 128 x 128, gate and up 132 us, where LDS is not read 125, without the DMA 78; 993 to 2 of 8
+// of 4096 x 11008, 256 x 256, 503, 498 and 383.  L2 sends 43 KB/us a CU in the first (1.36 GB) and 28 in the second; a line is on its way for 460 to 590 cycles,
+// 55 to 75 of them at a time, L1 waits for data in 41 to 60 % of its cycles and the matrix units are busy in 26 to 46 % of theirs; LDS banks never conflict.
 // Workgroups b, b + 8, ... run on one XCD and take a contiguous range of (expert, row block, token tile): both operands of neighbours are in its L2.
 template <typename T, int RTW_, int NTW_, int WR_, int WT_, int NST_ = 2, int UNIT_ = 16, bool PAIR_ = false> struct Grouped {
     static constexpr bool PAIR = PAIR_;
@@ -777,7 +778,7 @@ __global__ void __launch_bounds__(256) close_rows_kernel(CloseParams P) {
         store_vec<V>(reinterpret_cast<T *>(P.h) + (long long)t * P.ldh + at(c), v[c]);
     }
 }
-// rows of any length, which are read again for every step
+// rows of any length, which are read again for every step, an element a load: 2047 rows of 5120 107 us, of 11008 228 (1.2 TB/s)
 template <typename T>
 __global__ void __launch_bounds__(256) close_kernel(CloseParams P) {
     __shared__ float red[2][4];

@@ -70,12 +70,12 @@ hipError_t launch_route(const RouteParams &P, hipStream_t st) {
     return rc;
 }
 
-// Slot by slot where grouping hardly saves a matrix: one token, or half as many slots as experts (4 tokens to 8 of 64 of 1536 x 768 38 us, grouped 48;
-// 8 tokens 68 and 60.  2 tokens to 2 of 8 of 4096 x 11008 188 and 240, 4 tokens 349 and 280).
+// Slot by slot where grouping hardly saves a matrix: one token, or half as many slots as experts.  us a pass slot by slot and grouped: 1, 2, 4 and 8 tokens to 8
+// of 64 of 1536 x 768 15 and 29, 24 and 34, 41 and 53, 72 and 60; 1, 2 and 4 to 2 of 8 of 4096 x 11008 103 and 140, 212 and 207, 374 and 292.
 inline size_t most_by_token(int k, int experts) { return std::max(k, experts / 2); }
 // Up to so many tokens an expert on the average bfloat16 activations go on as pairs (what rounding leaves beside what it makes): the weights' way from memory hides
 // the second product.  us of it without and with: 64 experts of 1536 x 768, 4 tokens each 25 and 27, 16 each 31 and 37; 6 each of 1536 x 1024 33 and 35; 8 of 4096 x
-// 11008, 4 each 112 and 115, 16 each 139 and 171.  Error against 64 bits 2.35e-3 and 1.66e-3, which is the result's own rounding.
+// 11008, 4 each 117 and 118, 16 each 139 and 171.  Error against 64 bits 2.35e-3 and 1.66e-3, which is the result's own rounding.
 constexpr size_t PAIR_TOKENS = 8;
 ExpertsLayout experts_layout(int n, int k, int experts, int dim, int ff, int dtype) {
     const size_t slots = (size_t)n * k, es = dtype == NL_DTYPE_F32 ? 4 : 2;
@@ -139,16 +139,19 @@ template <bool FIRST, typename S> static double grouped_us(const ExpertsParams &
     return full * took(round) + (left > 0 ? took(left) : 0);
 }
 // Which tiles.  bfloat16: rows x tokens 64 x 64 in three stages (three workgroups a CU), 128 x 64 in two (three), 128 x 128 (two) or 256 x 256 (one), whichever
-// is expected to be done first: 1 % behind the best of the four on the average over 54 measured products.  us of a product with gate and up / with down:
+// is expected to be done first: over these products 1 % behind the best of the four on the average and 5 % at most.  us of a product with gate and up / with
+// down, the median of 24 over three sets of inputs (another run of the third line's 128 x 128 has 132 / 92: the chip's clock):
 //                                                                     64 x 64     128 x 64    128 x 128   256 x 256
-//   64 experts of 1536 x 768, 8 a token        32 tokens              49 / 27     49 / 25     61 / 32     74 / 40
-//                                              512                    82 / 47     78 / 47     76 / 47     87 / 53
-//                                              2047                   182 / 118   148 / 100   126 / 87    143 / 99
-//   64 of 1536 x 1024, 6 a token               64                     66 / 35     79 / 33     68 / 42     82 / 47
-//   8 of 768 x 2048, 2 a token                 333                    17 / 13     15 / 22     17 / 25     24 / 50
-//                                              1000                   33 / 21     30 / 30     30 / 33     29 / 56
-//   8 of 4096 x 11008, 2 a token               16                     224 / 108   215 / 152   237 / 155   259 / 209
-//                                              993                    783 / 431   634 / 409   559 / 447   587 / 335
+//   64 experts of 1536 x 768, 8 a token        32 tokens              50 / 28     48 / 25     60 / 32     73 / 40
+//                                              512                    80 / 47     78 / 47     75 / 46     85 / 53
+//                                              2047                   179 / 116   143 / 97    124 / 84    131 / 94
+//   64 of 1536 x 1024, 6 a token               64                     65 / 36     80 / 33     66 / 41     79 / 47
+//   8 of 768 x 2048, 2 a token                 333                    17 / 12     14 / 21     16 / 24     24 / 48
+//                                              1000                   32 / 20     28 / 29     29 / 32     28 / 55
+//   8 of 4096 x 11008, 2 a token               16                     221 / 117   232 / 149   243 / 149   252 / 209
+//                                              993                    732 / 399   572 / 354   505 / 361   500 / 278
+// (the last one's 256 x 256 take 431 or 503 by the inputs: an expert with a few tokens past 256 is another tile, and the last of them another round.  The rule
+// knows numbers, not the choices.)
 // 32 bits: 64 x 32 in three stages, bound by the matrix rate; 64 x 64 and 128 x 128 beside it: 77 tokens to 4 of 16 of 760 x 500 21 / 11, 22 / 15, 55 / 38; of the
 // first experts 256 tokens 166 / 87, 208 / 110, 385 / 198, 1024 tokens 507 / 260, 496 / 259, 596 / 319.
 template <typename T, bool FIRST> static hipError_t grouped_product(const ExpertsParams &P, hipStream_t st) {
@@ -184,8 +187,8 @@ template <typename T> static hipError_t experts(ExpertsParams P, bool &summed, h
         }
         return grouped_product<T, false>(P, st);
     }
-    // us a pass with rows on 16-byte boundaries, on 4-byte and on 2-byte ones: 333 tokens to 2 of 8 of 768 x 2048 32, 41, 499; 64 to 6 of 64 of 1536 x 1024
-    // 119, 125, 958; 2047 to 8 of 64 of 1536 x 768 251, 364, 7743
+    // us a pass with rows on 16-byte boundaries, on 4-byte and on 2-byte ones: 333 tokens to 2 of 8 of 768 x 2048 32, 43, 580; 64 to 6 of 64 of 1536 x 1024
+    // 111, 127, 871; 2047 to 8 of 64 of 1536 x 768 229, 393, 8425
     if (rows_on(4)) {
         if ((rc = grouped<T, true, Any<T>>(P, st)) != hipSuccess) return rc;
         return grouped<T, false, Any<T>>(P, st);
