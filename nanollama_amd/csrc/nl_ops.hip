@@ -183,6 +183,7 @@ template <typename T> static hipError_t experts(ExpertsParams P, bool &summed, h
         if (pair) P.h_rest = reinterpret_cast<T *>(P.h) + (size_t)slots * P.ff;
         if ((rc = grouped_product<T, true>(P, st)) != hipSuccess) return rc;
         if constexpr (sizeof(T) == 2) if (pair) {
+            // (reading the matrix bounds both: neither the second product nor the second half of the tokens' pieces is in the estimates)
             return grouped_us<false, PairLow<T>>(P, 5.4, 2.9) < grouped_us<false, PairSmall<T>>(P, 5.4, 2.9) ? grouped<T, false, PairLow<T>>(P, st) : grouped<T, false, PairSmall<T>>(P, st);
         }
         return grouped_product<T, false>(P, st);
